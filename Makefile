@@ -20,4 +20,4 @@ probes:
 	hipcc --offload-arch=gfx950 -O3 -std=c++17 -Wno-unused-value tools/elem_probe.hip -o tools/elem_probe
 
 clean:
-	rm -f cpd_amd/ops/_cpd_cpu.so cpd_amd/ops/_cpd_hip.so tools/gemm_probe tools/quant_gemm_probe tools/elem_probe
+	rm -rf cpd_amd/ops/_obj cpd_amd/ops/_cpd_cpu.so cpd_amd/ops/_cpd_hip.so tools/gemm_probe tools/quant_gemm_probe tools/elem_probe

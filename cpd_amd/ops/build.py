@@ -15,9 +15,11 @@ import os
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
+OBJ = os.path.join(HERE, "_obj")  # intermediate objects (not shipped)
 
 GFX_ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")
 
@@ -67,8 +69,30 @@ def _stale(target, sources):
     if not os.path.exists(target):
         return True
     t = os.path.getmtime(target)
-    deps = list(sources) + [os.path.join(CSRC, "quant_core.h"), __file__]
+    headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC)
+               if f.endswith(".h")]
+    deps = list(sources) + headers + [__file__]
     return any(os.path.getmtime(s) > t for s in deps)
+
+
+def _deps_of(obj):
+    """What the compiler's dependency file says ``obj`` was made from, or
+    None where there is none."""
+    try:
+        with open(obj[:-2] + ".d") as f:
+            names = f.read().replace("\\\n", " ").split(":", 1)[1].split()
+    except (OSError, IndexError):
+        return None
+    return [n for n in names if n.startswith(CSRC)]
+
+
+def _object_stale(obj, src):
+    deps = _deps_of(obj)
+    if deps is None or not os.path.exists(obj):
+        return True
+    t = os.path.getmtime(obj)
+    return any(not os.path.exists(s) or os.path.getmtime(s) > t
+               for s in deps + [src, __file__])
 
 
 def build_cpu(force=False, verbose=True):
@@ -101,21 +125,40 @@ def build_hip(force=False, verbose=True):
     if not force and not _stale(target, srcs):
         return target
     incs, libs, abi = _torch_paths()
-    cmd = (
+    # one object per source, compiled side by side: the host pass over
+    # torch's headers is most of a source's time
+    compile_flags = (
         ["hipcc", f"--offload-arch={GFX_ARCH}"]
-        + _common_flags("_cpd_hip", incs, abi)
+        + [f for f in _common_flags("_cpd_hip", incs, abi) if f != "-shared"]
         + [
             "-D__HIP_PLATFORM_AMD__=1",
             "-DUSE_ROCM=1",
             "-DHIPBLAS_V2",
             "-fno-gpu-rdc",
             "-Wno-unused-result",
+            # hipcc -O3 turns pairs of float operations into packed FP32
+            # instructions by itself; some of their forms give wrong results
+            # on gfx950, so the feature is off for all device code.  (The
+            # host pass warns that it does not know it: harmless.)
+            "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         ]
-        + srcs
-        + _link_flags(libs, hip=True)
-        + ["-o", target]
     )
-    _run(cmd, verbose)
+    os.makedirs(OBJ, exist_ok=True)
+    objs = [os.path.join(OBJ, os.path.basename(s) + ".o") for s in srcs]
+    todo = [(s, o) for s, o in zip(srcs, objs)
+            if force or _object_stale(o, s)]
+
+    def compile_one(job):
+        src, obj = job
+        _run(compile_flags + ["-MMD", "-MF", obj[:-2] + ".d", "-c", src,
+                              "-o", obj], verbose)
+
+    jobs = min(int(os.environ.get("MAX_JOBS", "8")), len(todo) or 1)
+    with ThreadPoolExecutor(max_workers=jobs) as pool:
+        list(pool.map(compile_one, todo))
+    _run(["hipcc", f"--offload-arch={GFX_ARCH}", "-shared", "-fPIC",
+          "-fno-gpu-rdc"] + objs + _link_flags(libs, hip=True)
+         + ["-o", target], verbose)
     return target
 
 
