@@ -3,6 +3,8 @@ kept, example/ResNet18/models/__init__.py:1)."""
 from .resnet_cifar import res_cifar, ResNetCifar
 from .resnet import resnet50, ResNet
 from .davidnet import davidnet, DavidNet
+from .fused_linear import FusedLinear, fused_linear
+from .fused_ln import FusedLayerNorm, fused_layer_norm
 
 def resnet50_quant(num_classes=1000, fused_bn=False, exp=5, man=2):
     """ResNet50 with every conv/linear GEMM routed through
@@ -34,4 +36,5 @@ def build_model(name, **kwargs):
 
 
 __all__ = ["res_cifar", "ResNetCifar", "resnet50", "ResNet", "davidnet",
-           "DavidNet", "build_model", "REGISTRY"]
+           "DavidNet", "build_model", "REGISTRY", "fused_layer_norm",
+           "FusedLayerNorm", "fused_linear", "FusedLinear"]

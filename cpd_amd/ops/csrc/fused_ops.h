@@ -1,0 +1,122 @@
+// Launchers of the layer-norm, linear and log-probability kernels.  Plain
+// pointers and sizes: the checks on tensors are in hip_bindings.cpp.  Each
+// enqueues on `stream` and returns; none allocates.
+#pragma once
+
+#include "fused_common.h"
+
+namespace cpd {
+
+struct NormArgs {
+  const void* x;          // [rows, cols], row stride x_ld
+  const void* res;        // or null
+  const void* weight;     // [cols] or null
+  const void* bias;       // [cols] or null
+  void* y;                // [rows, cols] contiguous
+  void* s;                // [rows, cols] contiguous, with res
+  float* stats;           // [rows, 2]: mean, 1/std; or null
+  long rows;
+  int cols;
+  long x_ld, res_ld;
+  float eps;
+  Dt dt, wdt;
+};
+void norm_forward(const NormArgs& a, hipStream_t stream);
+
+struct NormGradArgs {
+  const void* s;          // what was normalised [rows, cols], row stride s_ld
+  const void* dy;         // or null: zero
+  const void* ds;         // added to the result, or null
+  const void* weight;     // or null
+  const float* stats;     // [rows, 2]
+  void* dx;               // [rows, cols] contiguous
+  void* dweight;          // [cols] or null
+  void* dbias;            // [cols] or null
+  float* partial;         // [norm_grad_blocks(), 2, cols]
+  long rows;
+  int cols;
+  long s_ld, dy_ld, ds_ld;
+  Dt dt, wdt;
+};
+// How many rows of `partial` the backward pass writes for these sizes.
+int norm_grad_blocks(long rows, int cols, Dt dt);
+void norm_backward(const NormGradArgs& a, hipStream_t stream);
+
+constexpr int kMostTop = 64;  // alternatives: one lane of a wave each
+
+struct LogprobArgs {
+  const void* x;            // logits [rows, vocab], row stride ld
+  const int64_t* targets;   // [rows]
+  float* logprobs;          // [rows]
+  float* entropy;           // [rows]
+  float* stats;             // [rows, 2]: maximum, log of the sum around it
+  int64_t* top_ids;         // [rows, top] or null
+  float* top_logprobs;      // [rows, top] or null
+  void* work;               // logprob_work_bytes(), 8-byte aligned
+  long rows, ld;
+  int vocab, top;
+  int64_t ignore;
+  Dt dt;
+};
+long logprob_work_bytes(long rows, int vocab, int top, Dt dt);
+void logprob_forward(const LogprobArgs& a, hipStream_t stream);
+
+struct LogprobGradArgs {
+  const void* x;
+  const int64_t* targets;
+  const float* stats;       // of the forward pass
+  const float* entropy;
+  const float* glogprobs;   // [rows] or null
+  const float* gentropy;    // [rows] or null
+  void* dx;                 // [rows, vocab] contiguous
+  long rows, ld;
+  int vocab;
+  int64_t ignore;
+  Dt dt;
+};
+void logprob_backward(const LogprobGradArgs& a, hipStream_t stream);
+
+enum class Act : int { none = 0, relu = 1, gelu = 2, silu = 3 };
+
+// C[m, n] = sum over k of A(m, k) B(n, k), and what becomes of it.  An operand
+// lies with k innermost (A[m * ld + k]) or, `across`, with k outermost
+// (A[k * ld + m]).
+struct Operand {
+  const void* p;
+  long ld;
+  bool across;
+};
+struct GemmArgs {
+  Operand a, b;
+  int m, n, k;
+  Dt dt;              // of A, B, y, z, residual
+  void* y;            // [m, n], row stride y_ld: act(C + bias) + residual
+  long y_ld;
+  void* z;            // [m, n] contiguous: C + bias, or null
+  const void* bias;   // [n] or null
+  Dt bias_dt;
+  const void* res;    // [m, n], row stride res_ld, or null
+  long res_ld;
+  Act act;
+};
+void gemm_fused(const GemmArgs& a, hipStream_t stream);
+
+// dz = dy * act'(z) and the sums of its columns.
+struct ActGradArgs {
+  const void* dy;     // [m, n], row stride dy_ld
+  long dy_ld;
+  const void* z;      // [m, n], row stride z_ld; for relu the output may stand in
+  long z_ld;
+  void* dz;           // [m, n], row stride dz_ld, or null
+  long dz_ld;
+  void* dbias;        // [n] or null
+  Dt bias_dt;
+  float* partial;     // [act_grad_slices(), n], with dbias
+  int m, n;
+  Dt dt;
+  Act act;
+};
+int act_grad_slices(int m, int n, Dt dt);
+void act_grad(const ActGradArgs& a, hipStream_t stream);
+
+}  // namespace cpd

@@ -1,0 +1,471 @@
+// Tensors in, tensors out: checks, allocation and streams of the layer-norm,
+// linear and log-probability kernels.  Everything is enqueued on the current
+// stream of the tensors' device, whichever device is current; workspaces come
+// from torch's allocator in every call, so that two streams or two captured
+// graphs never share one.
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime.h>
+#include <torch/extension.h>
+
+#include <optional>
+#include <vector>
+
+#include "fused_ops.h"
+
+namespace {
+
+using at::Tensor;
+using cpd::Dt;
+using OptTensor = std::optional<Tensor>;
+using Guard = c10::hip::OptionalHIPGuardMasqueradingAsCUDA;
+
+Dt dtype_of(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kFloat:
+      return Dt::f32;
+    case at::kBFloat16:
+      return Dt::bf16;
+    case at::kHalf:
+      return Dt::f16;
+    default:
+      TORCH_CHECK_TYPE(false, name, " must be float32, bfloat16 or float16, got ",
+                       t.scalar_type());
+  }
+}
+
+void check_on(const Tensor& t, const Tensor& x, const char* name) {
+  TORCH_CHECK_VALUE(t.device() == x.device(), name, " is on ", t.device(),
+                    ", the input on ", x.device());
+}
+
+void check_like(const Tensor& t, const Tensor& x, const char* name) {
+  check_on(t, x, name);
+  TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type(), name, " is ",
+                   t.scalar_type(), ", the input ", x.scalar_type());
+  TORCH_CHECK_VALUE(t.sizes() == x.sizes(), name, " has shape ", t.sizes(),
+                    ", wanted ", x.sizes());
+}
+
+// A learned vector: contiguous, of the input's type or float32.
+std::optional<Tensor> learned(const OptTensor& t, const Tensor& x, int64_t n,
+                              const char* name) {
+  if (!t.has_value() || !t->defined()) return std::nullopt;
+  check_on(*t, x, name);
+  TORCH_CHECK_TYPE(
+      t->scalar_type() == x.scalar_type() || t->scalar_type() == at::kFloat,
+      name, " must be ", x.scalar_type(), " like the input, or float32, got ",
+      t->scalar_type());
+  TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == n, name, " has shape ",
+                    t->sizes(), ", wanted [", n, "]");
+  return t->contiguous();
+}
+
+// A tensor as rows of its last axis: itself where the rows are evenly apart
+// and their elements adjacent, a contiguous copy otherwise.
+struct Rows {
+  Tensor keep;
+  const void* p = nullptr;
+  long rows = 0, cols = 0, ld = 0;
+};
+
+Rows rows_of(const Tensor& t) {
+  Rows r;
+  r.cols = t.size(-1);
+  r.rows = r.cols ? t.numel() / r.cols : 0;
+  // Stride of the leading axes joined into one.  Axes that do not join, and
+  // rows that overlap (an expanded axis has stride 0), are copied.
+  long ld = r.cols, next = 0;
+  bool even = r.cols <= 1 || t.stride(-1) == 1, first = true;
+  for (int64_t d = t.dim() - 2; d >= 0 && even; --d) {
+    if (t.size(d) == 1) continue;
+    even = t.stride(d) >= r.cols && (first || t.stride(d) == next);
+    if (first) ld = t.stride(d);
+    next = t.stride(d) * t.size(d);
+    first = false;
+  }
+  if (!even) {
+    r.keep = t.contiguous();
+    ld = r.cols;
+  } else {
+    r.keep = t;
+  }
+  r.ld = ld;
+  r.p = r.keep.const_data_ptr();
+  return r;
+}
+
+hipStream_t stream_of(const Tensor& t) {
+  return c10::hip::getCurrentHIPStream(t.get_device()).stream();
+}
+
+void check_launch(const char* what) {
+  const hipError_t e = hipGetLastError();
+  TORCH_CHECK(e == hipSuccess, what, ": ", hipGetErrorString(e));
+}
+
+void check_input(const Tensor& x, const char* name) {
+  TORCH_CHECK_VALUE(x.is_cuda(), name, " must be on the GPU");
+}
+
+// ---------------------------------------------------------------------------
+// layer norm
+// ---------------------------------------------------------------------------
+
+// y, s (with a residual), stats [rows, 2]
+std::vector<Tensor> norm_fwd(const Tensor& x, const OptTensor& weight,
+                             const OptTensor& bias, double eps,
+                             const OptTensor& residual) {
+  check_input(x, "layer norm's input");
+  cpd::NormArgs a{};
+  a.dt = dtype_of(x, "layer norm's input");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1,
+                    "layer norm needs a last axis of one element or more");
+  TORCH_CHECK_VALUE(x.size(-1) < (1L << 30), "layer norm's last axis is too long");
+  const Guard guard(x.device());
+  const auto w = learned(weight, x, x.size(-1), "weight");
+  const auto b = learned(bias, x, x.size(-1), "bias");
+  TORCH_CHECK_TYPE(!w || !b || w->scalar_type() == b->scalar_type(),
+                   "weight and bias must have one type");
+  const Rows r = rows_of(x);
+  Rows q;
+  Tensor s;
+  if (residual.has_value()) {
+    check_like(*residual, x, "residual");
+    q = rows_of(*residual);
+    s = at::empty(x.sizes(), x.options());
+    a.res = q.p;
+    a.res_ld = q.ld;
+    a.s = s.mutable_data_ptr();
+  }
+  TORCH_CHECK_VALUE(r.rows < (1L << 31), "layer norm takes less than 2^31 rows");
+  TORCH_CHECK_VALUE(r.cols <= 16384 || r.rows < (1L << 22),
+                    "layer norm takes less than 2^22 rows of this length");
+  Tensor y = at::empty(x.sizes(), x.options());
+  Tensor stats = at::empty({r.rows, 2}, x.options().dtype(at::kFloat));
+  a.x = r.p;
+  a.x_ld = r.ld;
+  a.weight = w ? w->const_data_ptr() : nullptr;
+  a.bias = b ? b->const_data_ptr() : nullptr;
+  a.wdt = w ? dtype_of(*w, "weight") : b ? dtype_of(*b, "bias") : a.dt;
+  a.y = y.mutable_data_ptr();
+  a.stats = stats.data_ptr<float>();
+  a.rows = r.rows;
+  a.cols = (int)r.cols;
+  a.eps = (float)eps;
+  cpd::norm_forward(a, stream_of(x));
+  check_launch("layer norm");
+  return {y, s, stats};
+}
+
+// dx, dweight, dbias
+std::vector<Tensor> norm_bwd(const Tensor& s, const OptTensor& dy,
+                             const OptTensor& ds, const OptTensor& weight,
+                             const Tensor& stats, bool need_w, bool need_b,
+                             at::ScalarType bias_type) {
+  check_input(s, "layer norm's input");
+  const Guard guard(s.device());
+  cpd::NormGradArgs a{};
+  a.dt = dtype_of(s, "layer norm's input");
+  const Rows r = rows_of(s);
+  const auto w = learned(weight, s, r.cols, "weight");
+  TORCH_CHECK_VALUE(stats.is_contiguous() && stats.numel() == 2 * r.rows &&
+                        stats.scalar_type() == at::kFloat,
+                    "stats are not this input's");
+  check_on(stats, s, "stats");
+  Rows g, h;
+  if (dy.has_value() && dy->defined()) {
+    check_like(*dy, s, "the output's gradient");
+    g = rows_of(*dy);
+    a.dy = g.p;
+    a.dy_ld = g.ld;
+  }
+  if (ds.has_value() && ds->defined()) {
+    check_like(*ds, s, "the sum's gradient");
+    h = rows_of(*ds);
+    a.ds = h.p;
+    a.ds_ld = h.ld;
+  }
+  const auto wtype = w ? w->scalar_type() : bias_type;
+  const auto wopt = s.options().dtype(wtype);
+  Tensor dx = at::empty(s.sizes(), s.options());
+  Tensor dw, db, partial;
+  if (need_w || need_b) {
+    // no rows: the sums over them are zero
+    if (need_w) dw = r.rows ? at::empty({r.cols}, wopt) : at::zeros({r.cols}, wopt);
+    if (need_b) db = r.rows ? at::empty({r.cols}, wopt) : at::zeros({r.cols}, wopt);
+    partial = at::empty(
+        {cpd::norm_grad_blocks(r.rows, (int)r.cols, a.dt), 2, r.cols},
+        s.options().dtype(at::kFloat));
+    a.partial = partial.data_ptr<float>();
+  }
+  a.s = r.p;
+  a.s_ld = r.ld;
+  a.weight = w ? w->const_data_ptr() : nullptr;
+  a.stats = stats.data_ptr<float>();
+  a.dx = dx.mutable_data_ptr();
+  a.dweight = need_w ? dw.mutable_data_ptr() : nullptr;
+  a.dbias = need_b ? db.mutable_data_ptr() : nullptr;
+  a.rows = r.rows;
+  a.cols = (int)r.cols;
+  a.wdt = wtype == at::kFloat      ? Dt::f32
+          : wtype == at::kBFloat16 ? Dt::bf16
+                                   : Dt::f16;
+  cpd::norm_backward(a, stream_of(s));
+  check_launch("layer norm backward");
+  return {dx, dw, db};
+}
+
+// ---------------------------------------------------------------------------
+// log probabilities
+// ---------------------------------------------------------------------------
+
+// logprobs, entropy, stats, top_ids, top_logprobs
+std::vector<Tensor> logprob_fwd(const Tensor& x, const Tensor& targets,
+                                int64_t top, int64_t ignore) {
+  check_input(x, "logits");
+  cpd::LogprobArgs a{};
+  a.dt = dtype_of(x, "logits");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) < (1L << 30),
+                    "logits need a last axis of 1 to 2^30 - 1 entries");
+  check_on(targets, x, "targets");
+  TORCH_CHECK_TYPE(targets.scalar_type() == at::kLong, "targets must be int64, got ",
+                   targets.scalar_type());
+  TORCH_CHECK_VALUE(targets.sizes() == x.sizes().slice(0, x.dim() - 1),
+                    "targets have shape ", targets.sizes(), ", logits ", x.sizes());
+  TORCH_CHECK_VALUE(top >= 0 && top <= cpd::kMostTop && top <= x.size(-1),
+                    "top_k must be 0 to ", cpd::kMostTop,
+                    " and at most the number of logits, got ", top);
+  const Guard guard(x.device());
+  const Rows r = rows_of(x);
+  const Tensor t = targets.contiguous();
+  const auto f = x.options().dtype(at::kFloat);
+  Tensor lp = at::empty(t.sizes(), f), ent = at::empty(t.sizes(), f);
+  Tensor stats = at::empty({r.rows, 2}, f);
+  Tensor ids, tops, work;
+  if (top) {
+    auto shape = t.sizes().vec();
+    shape.push_back(top);
+    ids = at::empty(shape, t.options());
+    tops = at::empty(shape, f);
+  }
+  const long bytes = cpd::logprob_work_bytes(r.rows, (int)r.cols, (int)top, a.dt);
+  if (bytes) work = at::empty({bytes}, x.options().dtype(at::kByte));
+  a.x = r.p;
+  a.ld = r.ld;
+  a.targets = t.data_ptr<int64_t>();
+  a.logprobs = lp.data_ptr<float>();
+  a.entropy = ent.data_ptr<float>();
+  a.stats = stats.data_ptr<float>();
+  a.top_ids = top ? ids.mutable_data_ptr<int64_t>() : nullptr;
+  a.top_logprobs = top ? tops.data_ptr<float>() : nullptr;
+  a.work = bytes ? work.mutable_data_ptr() : nullptr;
+  a.rows = r.rows;
+  a.vocab = (int)r.cols;
+  a.top = (int)top;
+  a.ignore = ignore;
+  cpd::logprob_forward(a, stream_of(x));
+  check_launch("token log probabilities");
+  return {lp, ent, stats, ids, tops};
+}
+
+Tensor logprob_bwd(const Tensor& x, const Tensor& targets, const Tensor& stats,
+                   const Tensor& entropy, const OptTensor& glp,
+                   const OptTensor& gent, int64_t ignore) {
+  check_input(x, "logits");
+  const Guard guard(x.device());
+  cpd::LogprobGradArgs a{};
+  a.dt = dtype_of(x, "logits");
+  const Rows r = rows_of(x);
+  const Tensor t = targets.contiguous(), e = entropy.contiguous();
+  TORCH_CHECK_VALUE(t.numel() == r.rows && e.numel() == r.rows &&
+                        stats.numel() == 2 * r.rows && stats.is_contiguous(),
+                    "saved tensors are not these logits'");
+  Tensor g, h;
+  if (glp.has_value() && glp->defined()) g = glp->to(at::kFloat).contiguous();
+  if (gent.has_value() && gent->defined()) h = gent->to(at::kFloat).contiguous();
+  for (const Tensor* v : {&g, &h})
+    TORCH_CHECK_VALUE(!v->defined() || (v->device() == x.device() &&
+                                        v->numel() == r.rows),
+                      "a gradient does not fit the logits");
+  Tensor dx = at::empty(x.sizes(), x.options());
+  a.x = r.p;
+  a.ld = r.ld;
+  a.targets = t.data_ptr<int64_t>();
+  a.stats = stats.data_ptr<float>();
+  a.entropy = e.data_ptr<float>();
+  a.glogprobs = g.defined() ? g.data_ptr<float>() : nullptr;
+  a.gentropy = h.defined() ? h.data_ptr<float>() : nullptr;
+  a.dx = dx.mutable_data_ptr();
+  a.rows = r.rows;
+  a.vocab = (int)r.cols;
+  a.ignore = ignore;
+  cpd::logprob_backward(a, stream_of(x));
+  check_launch("token log probabilities backward");
+  return dx;
+}
+
+// ---------------------------------------------------------------------------
+// linear
+// ---------------------------------------------------------------------------
+
+constexpr int64_t kMostSize = (1L << 31) - 1024;
+
+cpd::Act act_of(int64_t act) {
+  TORCH_CHECK_VALUE(act >= 0 && act <= 3, "unknown activation");
+  return static_cast<cpd::Act>(act);
+}
+
+void check_sizes(int64_t m, int64_t n, int64_t k) {
+  TORCH_CHECK_VALUE(m < kMostSize && n < kMostSize && k < kMostSize,
+                    "linear takes sizes below 2^31 - 1024");
+  const int64_t tiles = ((m + 63) / 64) * ((n + 63) / 64);
+  TORCH_CHECK_VALUE(tiles < (1L << 24), "linear's output is too large");
+}
+
+// y, z (with want_z: act's argument, in the input's type)
+std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& weight,
+                               const OptTensor& bias, int64_t act,
+                               const OptTensor& residual, bool want_z) {
+  check_input(x, "linear's input");
+  cpd::GemmArgs g{};
+  g.dt = dtype_of(x, "linear's input");
+  g.act = act_of(act);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1),
+                    "linear's input has shape ", x.sizes(), ", its weight ",
+                    weight.sizes());
+  check_on(weight, x, "weight");
+  TORCH_CHECK_TYPE(weight.scalar_type() == x.scalar_type(), "weight is ",
+                   weight.scalar_type(), ", the input ", x.scalar_type());
+  TORCH_CHECK_VALUE(weight.size(1) >= 1, "linear needs one input feature or more");
+  const Guard guard(x.device());
+  const auto b = learned(bias, x, weight.size(0), "bias");
+  const Rows r = rows_of(x), w = rows_of(weight);
+  check_sizes(r.rows, weight.size(0), r.cols);
+  auto shape = x.sizes().vec();
+  shape.back() = weight.size(0);
+  Tensor y = at::empty(shape, x.options()), z;
+  Rows q;
+  if (residual.has_value()) {
+    check_like(*residual, y, "residual");
+    q = rows_of(*residual);
+    g.res = q.p;
+    g.res_ld = q.ld;
+  }
+  if (want_z) {
+    z = at::empty(shape, x.options());
+    g.z = z.mutable_data_ptr();
+  }
+  g.a = {r.p, r.ld, false};
+  g.b = {w.p, w.ld, false};
+  g.m = (int)r.rows;
+  g.n = (int)weight.size(0);
+  g.k = (int)r.cols;
+  g.y = y.mutable_data_ptr();
+  g.y_ld = g.n;
+  g.bias = b ? b->const_data_ptr() : nullptr;
+  g.bias_dt = b ? dtype_of(*b, "bias") : g.dt;
+  cpd::gemm_fused(g, stream_of(x));
+  check_launch("linear");
+  return {y, z};
+}
+
+// dx, dweight, dbias
+std::vector<Tensor> linear_bwd(const Tensor& dy, const Tensor& x,
+                               const Tensor& weight, const OptTensor& z,
+                               int64_t act, bool need_x, bool need_w,
+                               bool need_b, at::ScalarType bias_type) {
+  check_input(x, "linear's input");
+  const Guard guard(x.device());
+  const hipStream_t st = stream_of(x);
+  const Dt dt = dtype_of(x, "linear's input");
+  const int64_t n = weight.size(0), k = weight.size(1);
+  const Rows r = rows_of(x), w = rows_of(weight);
+  check_on(dy, x, "the output's gradient");
+  TORCH_CHECK_TYPE(dy.scalar_type() == x.scalar_type(), "the output's gradient is ",
+                   dy.scalar_type(), ", the input ", x.scalar_type());
+  TORCH_CHECK_VALUE(dy.size(-1) == n && dy.numel() == r.rows * n,
+                    "the output's gradient has shape ", dy.sizes());
+  const int64_t m = r.rows;
+  check_sizes(m, n, k);
+  check_sizes(m, k, n);
+  check_sizes(n, k, m);
+  Rows g = rows_of(dy);
+  g.rows = m;
+  Tensor dx, dw, db, dz, partial;
+  if (need_x) dx = at::empty(x.sizes(), x.options());
+  if (need_w) dw = m ? at::empty({n, k}, x.options()) : at::zeros({n, k}, x.options());
+  const auto bopt = x.options().dtype(bias_type);
+  if (need_b) db = m ? at::empty({n}, bopt) : at::zeros({n}, bopt);
+  if (m == 0 || n == 0) {
+    if (need_x && n == 0) dx.zero_();
+    return {dx, dw, db};
+  }
+  cpd::ActGradArgs p{};
+  p.act = act_of(act);
+  p.dt = dt;
+  p.m = (int)m;
+  p.n = (int)n;
+  p.dy = g.p;
+  p.dy_ld = g.ld;
+  Rows zr;
+  if (p.act != cpd::Act::none) {
+    TORCH_CHECK_VALUE(z.has_value() && z->numel() == m * n, "linear kept no z");
+    zr = rows_of(*z);
+    p.z = zr.p;
+    p.z_ld = zr.ld;
+    if (need_x || need_w) {
+      dz = at::empty({m, n}, x.options());
+      p.dz = dz.mutable_data_ptr();
+      p.dz_ld = n;
+      g.p = p.dz;
+      g.ld = n;
+    }
+  }
+  if (need_b) {
+    p.dbias = db.mutable_data_ptr();
+    p.bias_dt = bias_type == at::kFloat ? Dt::f32 : dt;
+    partial = at::empty({cpd::act_grad_slices(p.m, p.n, dt), n},
+                        x.options().dtype(at::kFloat));
+    p.partial = partial.data_ptr<float>();
+  }
+  if (need_b || p.dz) cpd::act_grad(p, st);
+  cpd::GemmArgs a{};
+  a.dt = a.bias_dt = dt;
+  if (need_x) {  // dz [m, n] with W [n, k]: the sum runs over n
+    a.a = {g.p, g.ld, false};
+    a.b = {w.p, w.ld, true};
+    a.m = (int)m;
+    a.n = (int)k;
+    a.k = (int)n;
+    a.y = dx.mutable_data_ptr();
+    a.y_ld = k;
+    cpd::gemm_fused(a, st);
+  }
+  if (need_w) {  // dz^T x: the sum runs over m
+    a.a = {g.p, g.ld, true};
+    a.b = {r.p, r.ld, true};
+    a.m = (int)n;
+    a.n = (int)k;
+    a.k = (int)m;
+    a.y = dw.mutable_data_ptr();
+    a.y_ld = k;
+    cpd::gemm_fused(a, st);
+  }
+  check_launch("linear backward");
+  return {dx, dw, db};
+}
+
+}  // namespace
+
+void cpd_register_fused(pybind11::module_& m) {
+  m.def("norm_fwd", &norm_fwd,
+        "layer norm (+residual): returns (y, s, stats)");
+  m.def("norm_bwd", &norm_bwd,
+        "layer norm backward: returns (dx, dweight, dbias)");
+  m.def("logprob_fwd", &logprob_fwd,
+        "returns (logprobs, entropy, stats, top_ids, top_logprobs)");
+  m.def("logprob_bwd", &logprob_bwd, "gradient of the logits");
+  m.def("linear_fwd", &linear_fwd, "act(x W^T + b) + residual: (y, z)");
+  m.def("linear_bwd", &linear_bwd, "returns (dx, dweight, dbias)");
+}

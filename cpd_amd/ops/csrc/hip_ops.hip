@@ -607,9 +607,11 @@ at::Tensor cpd_quant_gemm_hip(const at::Tensor& a, const at::Tensor& b,
                               int64_t man, int64_t exp);
 at::Tensor cpd_gemm_f32_hip(const at::Tensor& a, const at::Tensor& b);
 void cpd_register_bn(pybind11::module_& m);
+void cpd_register_fused(pybind11::module_& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   cpd_register_bn(m);
+  cpd_register_fused(m);
   m.def("quantize", &quantize);
   m.def("quantize_", &quantize_);
   m.def("qadd_", &qadd_);
