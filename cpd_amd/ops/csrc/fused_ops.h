@@ -85,6 +85,7 @@ struct Operand {
   const void* p;
   long ld;
   bool across;
+  bool padded;  // across: a row's last 8 elements may be read past its end
 };
 struct GemmArgs {
   Operand a, b;
@@ -98,7 +99,14 @@ struct GemmArgs {
   const void* res;    // [m, n], row stride res_ld, or null
   long res_ld;
   Act act;
+  float* work;        // gemm_work_floats()
 };
+long gemm_work_floats(long m, long n, long k, Dt dt);
+// Whether a 16-bit product takes the operand as it lies (`rows` by k), 16
+// bytes at a time; if not, pad_rows makes a copy that it takes.
+bool gemm_takes(const Operand& o, long rows);
+void pad_rows(const void* from, long ld, void* to, long to_ld, int rows,
+              int cols, Dt dt, hipStream_t stream);
 void gemm_fused(const GemmArgs& a, hipStream_t stream);
 
 // dz = dy * act'(z) and the sums of its columns.

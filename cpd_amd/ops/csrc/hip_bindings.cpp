@@ -321,14 +321,45 @@ void check_sizes(int64_t m, int64_t n, int64_t k) {
                     "linear takes sizes below 2^31 - 1024");
   const int64_t tiles = ((m + 63) / 64) * ((n + 63) / 64);
   TORCH_CHECK_VALUE(tiles < (1L << 24), "linear's output is too large");
+  // (a tile's 256 rows are reached with 32-bit offsets)
+  TORCH_CHECK_VALUE(n < (1L << 22) && k < (1L << 22),
+                    "linear takes less than 2^22 features");
 }
+
+// What one product needs beside its operands; kept until it is enqueued.
+struct Product {
+  cpd::GemmArgs g{};
+  Tensor keep[3];
+
+  // An operand, as it lies or copied to where 16-byte reads fit.
+  cpd::Operand operand(const Rows& r, bool across, bool padded, int which) {
+    cpd::Operand o{r.p, r.ld, across, padded};
+    if (g.dt == Dt::f32 || r.rows == 0 ||
+        cpd::gemm_takes(o, across ? r.cols : r.rows))
+      return o;
+    const int64_t ld = (r.cols + 7) / 8 * 8;
+    keep[which] = at::empty({r.rows, ld}, r.keep.options());
+    cpd::pad_rows(r.p, r.ld, keep[which].mutable_data_ptr(), ld, (int)r.rows,
+                  (int)r.cols, g.dt, stream_of(r.keep));
+    return {keep[which].const_data_ptr(), ld, across, true};
+  }
+  void run(const Tensor& like) {
+    const long floats = cpd::gemm_work_floats(g.m, g.n, g.k, g.dt);
+    if (floats) {
+      keep[2] = at::empty({floats}, like.options().dtype(at::kFloat));
+      g.work = keep[2].data_ptr<float>();
+    }
+    cpd::gemm_fused(g, stream_of(like));
+  }
+};
 
 // y, z (with want_z: act's argument, in the input's type)
 std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& weight,
                                const OptTensor& bias, int64_t act,
                                const OptTensor& residual, bool want_z) {
   check_input(x, "linear's input");
-  cpd::GemmArgs g{};
+  Product product;
+  cpd::GemmArgs& g = product.g;
   g.dt = dtype_of(x, "linear's input");
   g.act = act_of(act);
   TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1),
@@ -356,8 +387,8 @@ std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& weight,
     z = at::empty(shape, x.options());
     g.z = z.mutable_data_ptr();
   }
-  g.a = {r.p, r.ld, false};
-  g.b = {w.p, w.ld, false};
+  g.a = product.operand(r, false, false, 0);
+  g.b = product.operand(w, false, false, 1);
   g.m = (int)r.rows;
   g.n = (int)weight.size(0);
   g.k = (int)r.cols;
@@ -365,7 +396,7 @@ std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& weight,
   g.y_ld = g.n;
   g.bias = b ? b->const_data_ptr() : nullptr;
   g.bias_dt = b ? dtype_of(*b, "bias") : g.dt;
-  cpd::gemm_fused(g, stream_of(x));
+  product.run(x);
   check_launch("linear");
   return {y, z};
 }
@@ -415,11 +446,13 @@ std::vector<Tensor> linear_bwd(const Tensor& dy, const Tensor& x,
     p.z = zr.p;
     p.z_ld = zr.ld;
     if (need_x || need_w) {
-      dz = at::empty({m, n}, x.options());
+      // rows a multiple of 16 bytes apart, as the products read them
+      g.ld = (n + 7) / 8 * 8;
+      dz = at::empty({m, g.ld}, x.options());
       p.dz = dz.mutable_data_ptr();
-      p.dz_ld = n;
+      p.dz_ld = g.ld;
       g.p = p.dz;
-      g.ld = n;
+      g.keep = dz;
     }
   }
   if (need_b) {
@@ -430,27 +463,29 @@ std::vector<Tensor> linear_bwd(const Tensor& dy, const Tensor& x,
     p.partial = partial.data_ptr<float>();
   }
   if (need_b || p.dz) cpd::act_grad(p, st);
-  cpd::GemmArgs a{};
-  a.dt = a.bias_dt = dt;
   if (need_x) {  // dz [m, n] with W [n, k]: the sum runs over n
-    a.a = {g.p, g.ld, false};
-    a.b = {w.p, w.ld, true};
-    a.m = (int)m;
-    a.n = (int)k;
-    a.k = (int)n;
-    a.y = dx.mutable_data_ptr();
-    a.y_ld = k;
-    cpd::gemm_fused(a, st);
+    Product q;
+    q.g.dt = q.g.bias_dt = dt;
+    q.g.a = q.operand(g, false, p.dz != nullptr, 0);
+    q.g.b = q.operand(w, true, false, 1);
+    q.g.m = (int)m;
+    q.g.n = (int)k;
+    q.g.k = (int)n;
+    q.g.y = dx.mutable_data_ptr();
+    q.g.y_ld = k;
+    q.run(x);
   }
   if (need_w) {  // dz^T x: the sum runs over m
-    a.a = {g.p, g.ld, true};
-    a.b = {r.p, r.ld, true};
-    a.m = (int)n;
-    a.n = (int)k;
-    a.k = (int)m;
-    a.y = dw.mutable_data_ptr();
-    a.y_ld = k;
-    cpd::gemm_fused(a, st);
+    Product q;
+    q.g.dt = q.g.bias_dt = dt;
+    q.g.a = q.operand(g, true, p.dz != nullptr, 0);
+    q.g.b = q.operand(r, true, false, 1);
+    q.g.m = (int)n;
+    q.g.n = (int)k;
+    q.g.k = (int)m;
+    q.g.y = dw.mutable_data_ptr();
+    q.g.y_ld = k;
+    q.run(x);
   }
   check_launch("linear backward");
   return {dx, dw, db};
