@@ -70,6 +70,21 @@ __device__ __forceinline__ void load_some(const T* p, int left, float* out) {
   }
 }
 
+template <typename T, int N>
+__device__ __forceinline__ void store_some(T* p, int left, const float* in) {
+  typedef T V __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+  if (left >= N) {
+    V v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (T)in[i];
+    *reinterpret_cast<V*>(p) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < left) p[i] = (T)in[i];
+  }
+}
+
 // N elements of a vector whose type is known at run time only (weights and
 // biases: the activations' type, or float).
 template <int N>

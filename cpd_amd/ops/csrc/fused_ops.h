@@ -101,10 +101,13 @@ struct GemmArgs {
   Act act;
   float* work;        // gemm_work_floats()
 };
-long gemm_work_floats(long m, long n, long k, Dt dt);
+// `along`: both operands are
+long gemm_work_floats(long m, long n, long k, Dt dt, bool along);
 // Whether a 16-bit product takes the operand as it lies (`rows` by k), 16
-// bytes at a time; if not, pad_rows makes a copy that it takes.
+// bytes at a time; if not, pad_rows makes a copy that it takes.  Floats are
+// taken as they lie, and so is everything along with gemm_few_rows.
 bool gemm_takes(const Operand& o, long rows);
+bool gemm_few_rows(long m, long n, long k, Dt dt);
 void pad_rows(const void* from, long ld, void* to, long to_ld, int rows,
               int cols, Dt dt, hipStream_t stream);
 void gemm_fused(const GemmArgs& a, hipStream_t stream);

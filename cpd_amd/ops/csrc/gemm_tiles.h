@@ -57,12 +57,7 @@ __device__ __forceinline__ void copy_to_lds(const void* base, u32 off, u32 lds) 
 
 template <int N>
 __device__ __forceinline__ void wait_copies() {  // all but the newest N, and LDS reads
-  if constexpr (N == 0)
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  else if constexpr (N == 10)
-    asm volatile("s_waitcnt vmcnt(10) lgkmcnt(0)" ::: "memory");
-  else
-    static_assert(N == 0 || N == 10, "a count that has no instruction here");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ void block_barrier() {
@@ -80,6 +75,8 @@ __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(
         __builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
+
+__device__ __forceinline__ int swizzle_along(int r) { return r >> 1 & 7; }
 
 __device__ __forceinline__ int swizzle_across(int k) {
   return 2 * ((k & 3) | ((k >> 3) & 1) << 2);
@@ -111,7 +108,7 @@ struct Copier {
 #pragma unroll
       for (int i = 0; i < PASSES; ++i) {
         const int r = (i * WAVES + wave) * 8 + (lane >> 3);
-        const int chunk = (lane & 7) ^ ((r >> 1) & 7);
+        const int chunk = (lane & 7) ^ swizzle_along(r);
         at[i] = chunk * 8;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -138,17 +135,17 @@ struct Copier {
     }
   }
 
-  __device__ __forceinline__ void half(long tile, int h, u32 lds) const {
-    const char* b = base + tile * step;
+  __device__ __forceinline__ void half(int tile, int h, u32 lds) const {
+    const char* b = base + (long)tile * step;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i)
       copy_to_lds(b, off[h][i], lds + place + i * (WAVES * 1024));
   }
 
   // The last tile, of `left` < 64 k: through registers, zeros behind its end.
-  __device__ __forceinline__ void rest(long tile, int h, char* lds, int left,
+  __device__ __forceinline__ void rest(int tile, int h, char* lds, int left,
                                        int lane) const {
-    const char* b = base + tile * step;
+    const char* b = base + (long)tile * step;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       s16x8 v = {};
@@ -174,7 +171,7 @@ __device__ __forceinline__ s16x8 fragment(const char* half, int row, int kk,
                                           int lane) {
   if constexpr (!ACROSS) {
     const int r = row + (lane & 15);
-    const int place = (kk * 4 + (lane >> 4)) ^ ((r >> 1) & 7);
+    const int place = (kk * 4 + (lane >> 4)) ^ swizzle_along(r);
     return *reinterpret_cast<const s16x8*>(half + r * 128 + place * 16);
   } else {
     const int s = lane & 15;
@@ -188,16 +185,130 @@ __device__ __forceinline__ s16x8 fragment(const char* half, int row, int kk,
   }
 }
 
-// A wave's 64 by 64 results, v[i][j] for rows 16 i + lane % 16 and columns
-// 16 j + 4 (lane / 16), through 16 KB of LDS of its own (a row's 16-byte
-// chunks in the order chunk ^ row % 16, which keeps both sides off each
-// other's banks).  `put(row, col, v)` then gets eight neighbouring results;
-// eight lanes have a row's 64.
-template <typename F>
-__device__ __forceinline__ void leave(char* lds, f32x4 (&v)[4][4], int lane,
-                                      F put) {
+// ---------------------------------------------------------------------------
+// Floats on the 16-bit matrix cores.
+//
+// A float is the sum of three bf16, exactly: each takes the next eight bits of
+// its significand (cut off, not rounded, so that nothing overflows).  Of the
+// nine products of two floats' parts the six largest are kept,
+//   a1 b1 + (a1 b2 + a2 b1) + (a1 b3 + a2 b2 + a3 b1),
+// the rest is below 2^-24 of a b.  At a sixth of the 16-bit rate that is more
+// than twice the float matrix instructions' 157 TFLOP/s.
+//
+// What is not finite becomes (+-1, 0, x): the third part meets first parts
+// only, which are zero for zeros alone, so inf times 0 is NaN, inf times
+// anything else inf, and no part of a finite number makes a NaN of it.
+// (Floats below the normal range count as zero.)
+//
+// Tiles are of 32 k and three planes of 8 KB: along, row r of 64 bytes with
+// its chunk c at place c ^ r/2 % 4; across, as above.
+__device__ __forceinline__ int swizzle_float(int r) { return r >> 1 & 3; }
+
+constexpr int kFloatK = 32;
+constexpr int kPlane = 8192;
+
+// One thread's share of 128 rows by 32 k: eight floats.
+template <bool ACROSS>
+struct FloatStager {
+  const float* p;  // of this thread's eight, in the first tile
+  long step;       // floats from a tile to the next
+  int at;          // along: its first k; across: its k
+  int rows_left;   // across: rows from its first on
+  u32 place;       // where its 16 bytes of a plane belong
+
+  __device__ __forceinline__ void start(const Operand& o, int row0, int rows,
+                                        int tid) {  // of 512
+    const float* base = static_cast<const float*>(o.p);
+    if constexpr (!ACROSS) {
+      const int r = tid >> 2, chunk = tid & 3;
+      at = chunk * 8;
+      rows_left = 8;
+      p = base + (long)min(row0 + r, rows - 1) * o.ld + at;
+      step = kFloatK;
+      place = r * 64 + ((chunk ^ swizzle_float(r)) << 4);
+    } else {
+      const int chunk = tid & 15;
+      at = tid >> 4;
+      rows_left = rows - (row0 + chunk * 8);
+      p = base + (long)at * o.ld + row0 + chunk * 8;
+      step = kFloatK * o.ld;
+      place = at * 256 + ((chunk ^ swizzle_across(at)) << 4);
+    }
+  }
+
+  // `left`: k from this tile's first on
+  __device__ __forceinline__ void load(int tile, int left, float (&v)[8]) const {
+    const float* q = p + tile * step;
+    const int n = ACROSS ? (at < left ? rows_left : 0) : left - at;
+    load_some<float, 8>(q, n, v);
+  }
+
+  __device__ __forceinline__ void store(char* lds, const float (&v)[8]) const {
+    u32 part[3][4];
+    u32 most = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i]) << 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u32 first[2], second[2], third[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float x = v[2 * i + j];
+        first[j] = __float_as_uint(x) & 0xFFFF0000u;
+        const float r = x - __uint_as_float(first[j]);
+        second[j] = __float_as_uint(r) & 0xFFFF0000u;
+        third[j] = __float_as_uint(r - __uint_as_float(second[j]));
+      }
+      // the upper halves of two, side by side
+      part[0][i] = __builtin_amdgcn_perm(first[1], first[0], 0x07060302u);
+      part[1][i] = __builtin_amdgcn_perm(second[1], second[0], 0x07060302u);
+      part[2][i] = __builtin_amdgcn_perm(third[1], third[0], 0x07060302u);
+    }
+    if (most >= 0xFF000000u) {  // an infinity or NaN among the eight
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const u32 u = __float_as_uint(v[i]);
+        if ((u << 1) < 0xFF000000u) continue;
+        const u32 sh = (i & 1) * 16, keep = i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+        // (a NaN whose bits are all in the lower half must stay one)
+        const u32 top = (u >> 16) | (u << 9 ? 0x40u : 0u);
+        part[0][i / 2] = (part[0][i / 2] & keep) |
+                         ((0x3F80u | (u >> 16 & 0x8000u)) << sh);
+        part[1][i / 2] = part[1][i / 2] & keep;
+        part[2][i / 2] = (part[2][i / 2] & keep) | (top << sh);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+      typedef u32 V __attribute__((ext_vector_type(4)));
+      *reinterpret_cast<V*>(lds + q * kPlane + place) =
+          V{part[q][0], part[q][1], part[q][2], part[q][3]};
+    }
+  }
+};
+
+template <bool ACROSS>
+__device__ __forceinline__ s16x8 float_fragment(const char* plane, int row,
+                                                int lane) {
+  if constexpr (!ACROSS) {
+    const int r = row + (lane & 15);
+    const int place = (lane >> 4) ^ swizzle_float(r);
+    return *reinterpret_cast<const s16x8*>(plane + r * 64 + place * 16);
+  } else {
+    return fragment<true>(plane, row, 0, lane);
+  }
+}
+
+// A wave's results, 16 F rows by 64, v[i][j] for rows 16 i + lane % 16 and
+// columns 16 j + 4 (lane / 16), through 4 F KB of LDS of its own (a row's
+// 16-byte chunks in the order chunk ^ row % 16, which keeps both sides off
+// each other's banks).  `put(row, col, v)` then gets eight neighbouring
+// results; eight lanes have a row's 64.
+template <int F, typename P>
+__device__ __forceinline__ void leave(char* lds, const f32x4 (*v)[4], int lane,
+                                      P put) {
+#pragma unroll
+  for (int i = 0; i < F; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int row = i * 16 + (lane & 15), chunk = j * 4 + (lane >> 4);
@@ -205,7 +316,7 @@ __device__ __forceinline__ void leave(char* lds, f32x4 (&v)[4][4], int lane,
           v[i][j];
     }
 #pragma unroll 1
-  for (int pass = 0; pass < 8; ++pass) {
+  for (int pass = 0; pass < 2 * F; ++pass) {
     const int row = pass * 8 + (lane >> 3), chunk = (lane & 7) * 2;
     const f32x4 lo = *reinterpret_cast<const f32x4*>(
         lds + row * 256 + ((chunk ^ (row & 15)) << 4));

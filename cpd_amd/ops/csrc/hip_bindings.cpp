@@ -326,30 +326,34 @@ void check_sizes(int64_t m, int64_t n, int64_t k) {
                     "linear takes less than 2^22 features");
 }
 
-// What one product needs beside its operands; kept until it is enqueued.
-struct Product {
-  cpd::GemmArgs g{};
-  Tensor keep[3];
+// The products of a call: operands as the kernels read them, and workspaces,
+// kept until all is enqueued.
+struct Products {
+  Dt dt;
+  hipStream_t st;
+  std::vector<Tensor> keep;
 
-  // An operand, as it lies or copied to where 16-byte reads fit.
-  cpd::Operand operand(const Rows& r, bool across, bool padded, int which) {
+  cpd::Operand operand(const Rows& r, bool across, bool padded, bool few,
+                       const Tensor& like) {
     cpd::Operand o{r.p, r.ld, across, padded};
-    if (g.dt == Dt::f32 || r.rows == 0 ||
+    if (few || dt == Dt::f32 || r.rows == 0 ||
         cpd::gemm_takes(o, across ? r.cols : r.rows))
       return o;
     const int64_t ld = (r.cols + 7) / 8 * 8;
-    keep[which] = at::empty({r.rows, ld}, r.keep.options());
-    cpd::pad_rows(r.p, r.ld, keep[which].mutable_data_ptr(), ld, (int)r.rows,
-                  (int)r.cols, g.dt, stream_of(r.keep));
-    return {keep[which].const_data_ptr(), ld, across, true};
+    keep.push_back(at::empty({r.rows, ld}, like.options()));
+    cpd::pad_rows(r.p, r.ld, keep.back().mutable_data_ptr(), ld, (int)r.rows,
+                  (int)r.cols, dt, st);
+    return {keep.back().const_data_ptr(), ld, across, true};
   }
-  void run(const Tensor& like) {
-    const long floats = cpd::gemm_work_floats(g.m, g.n, g.k, g.dt);
+
+  void run(cpd::GemmArgs& g, const Tensor& like) {
+    const long floats = cpd::gemm_work_floats(g.m, g.n, g.k, dt,
+                                              !g.a.across && !g.b.across);
     if (floats) {
-      keep[2] = at::empty({floats}, like.options().dtype(at::kFloat));
-      g.work = keep[2].data_ptr<float>();
+      keep.push_back(at::empty({floats}, like.options().dtype(at::kFloat)));
+      g.work = keep.back().data_ptr<float>();
     }
-    cpd::gemm_fused(g, stream_of(like));
+    cpd::gemm_fused(g, st);
   }
 };
 
@@ -358,8 +362,7 @@ std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& weight,
                                const OptTensor& bias, int64_t act,
                                const OptTensor& residual, bool want_z) {
   check_input(x, "linear's input");
-  Product product;
-  cpd::GemmArgs& g = product.g;
+  cpd::GemmArgs g{};
   g.dt = dtype_of(x, "linear's input");
   g.act = act_of(act);
   TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1),
@@ -387,8 +390,10 @@ std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& weight,
     z = at::empty(shape, x.options());
     g.z = z.mutable_data_ptr();
   }
-  g.a = product.operand(r, false, false, 0);
-  g.b = product.operand(w, false, false, 1);
+  Products products{g.dt, stream_of(x), {}};
+  const bool few = cpd::gemm_few_rows(r.rows, w.rows, r.cols, g.dt);
+  g.a = products.operand(r, false, false, few, x);
+  g.b = products.operand(w, false, false, few, x);
   g.m = (int)r.rows;
   g.n = (int)weight.size(0);
   g.k = (int)r.cols;
@@ -396,7 +401,7 @@ std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& weight,
   g.y_ld = g.n;
   g.bias = b ? b->const_data_ptr() : nullptr;
   g.bias_dt = b ? dtype_of(*b, "bias") : g.dt;
-  product.run(x);
+  products.run(g, x);
   check_launch("linear");
   return {y, z};
 }
@@ -463,29 +468,29 @@ std::vector<Tensor> linear_bwd(const Tensor& dy, const Tensor& x,
     p.partial = partial.data_ptr<float>();
   }
   if (need_b || p.dz) cpd::act_grad(p, st);
-  if (need_x) {  // dz [m, n] with W [n, k]: the sum runs over n
-    Product q;
-    q.g.dt = q.g.bias_dt = dt;
-    q.g.a = q.operand(g, false, p.dz != nullptr, 0);
-    q.g.b = q.operand(w, true, false, 1);
-    q.g.m = (int)m;
-    q.g.n = (int)k;
-    q.g.k = (int)n;
-    q.g.y = dx.mutable_data_ptr();
-    q.g.y_ld = k;
-    q.run(x);
+  // dx: dz [m, n] with W [n, k], the sum runs over n;
+  // dW: dz^T x, the sum runs over m
+  Products products{dt, st, {}};
+  const bool padded = p.dz != nullptr;
+  cpd::GemmArgs q{};
+  q.dt = q.bias_dt = dt;
+  q.n = (int)k;
+  q.y_ld = k;
+  if (need_x) {
+    q.a = products.operand(g, false, padded, false, x);
+    q.b = products.operand(w, true, false, false, x);
+    q.m = (int)m;
+    q.k = (int)n;
+    q.y = dx.mutable_data_ptr();
+    products.run(q, x);
   }
-  if (need_w) {  // dz^T x: the sum runs over m
-    Product q;
-    q.g.dt = q.g.bias_dt = dt;
-    q.g.a = q.operand(g, true, p.dz != nullptr, 0);
-    q.g.b = q.operand(r, true, false, 1);
-    q.g.m = (int)n;
-    q.g.n = (int)k;
-    q.g.k = (int)m;
-    q.g.y = dw.mutable_data_ptr();
-    q.g.y_ld = k;
-    q.run(x);
+  if (need_w) {
+    q.a = products.operand(g, true, padded, false, x);
+    q.b = products.operand(r, true, false, false, x);
+    q.m = (int)n;
+    q.k = (int)m;
+    q.y = dw.mutable_data_ptr();
+    products.run(q, x);
   }
   check_launch("linear backward");
   return {dx, dw, db};

@@ -44,143 +44,8 @@ __device__ __forceinline__ float act_slope(float z, Act act) {
   }
 }
 
-// y and z of one element.
-template <typename T>
-__device__ __forceinline__ void finish(const GemmArgs& g, int row, int col,
-                                       float v, float bias) {
-  v += bias;
-  if (g.z) static_cast<T*>(g.z)[(long)row * g.n + col] = (T)v;
-  v = act_value(v, g.act);
-  if (g.res)
-    v += (float)static_cast<const T*>(g.res)[(long)row * g.res_ld + col];
-  static_cast<T*>(g.y)[(long)row * g.y_ld + col] = (T)v;
-}
-
 // ---------------------------------------------------------------------------
-// Any sizes, strides and alignment: 64x64 tile, four waves of 32x32.
-// ---------------------------------------------------------------------------
-
-template <typename T>
-constexpr int kAnyK = 64 / sizeof(T);  // k of a tile: 64 bytes
-
-// A 64-row tile of an operand into LDS as [row][k]; zeros behind its ends.
-template <typename T>
-__device__ __forceinline__ void any_stage(const Operand& o, int row0, int rows,
-                                          int k0, int k,
-                                          T (*to)[kAnyK<T> + 16 / sizeof(T)]) {
-  constexpr int BK = kAnyK<T>, VEC = 16 / sizeof(T);
-  const T* p = static_cast<const T*>(o.p);
-  typedef T V __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
-  // 64 * BK elements, one vector a thread
-  if (!o.across) {
-    const int r = threadIdx.x / (BK / VEC), c = threadIdx.x % (BK / VEC) * VEC;
-    const int left = row0 + r < rows ? k - (k0 + c) : 0;
-    const T* at = p + (long)(row0 + r) * o.ld + k0 + c;
-    V v = {};
-    if (left >= VEC) {
-      v = *reinterpret_cast<const V*>(at);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (i < left) v[i] = at[i];
-    }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) to[r][c + i] = v[i];
-  } else {
-    const int kk = threadIdx.x / (64 / VEC), r = threadIdx.x % (64 / VEC) * VEC;
-    const int left = k0 + kk < k ? rows - (row0 + r) : 0;
-    const T* at = p + (long)(k0 + kk) * o.ld + row0 + r;
-    V v = {};
-    if (left >= VEC) {
-      v = *reinterpret_cast<const V*>(at);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (i < left) v[i] = at[i];
-    }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) to[r + i][kk] = v[i];
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ f32x4 mfma_row(const T* a, const T* b, int lane,
-                                          f32x4 c);
-template <>
-__device__ __forceinline__ f32x4 mfma_row<bf16_t>(const bf16_t* a,
-                                                  const bf16_t* b, int lane,
-                                                  f32x4 c) {
-  const int k = (lane >> 4) * 8;
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-      *reinterpret_cast<const bf16x8*>(a + k),
-      *reinterpret_cast<const bf16x8*>(b + k), c, 0, 0, 0);
-}
-template <>
-__device__ __forceinline__ f32x4 mfma_row<f16_t>(const f16_t* a,
-                                                 const f16_t* b, int lane,
-                                                 f32x4 c) {
-  const int k = (lane >> 4) * 8;
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(
-      *reinterpret_cast<const f16x8*>(a + k),
-      *reinterpret_cast<const f16x8*>(b + k), c, 0, 0, 0);
-}
-template <>
-__device__ __forceinline__ f32x4 mfma_row<float>(const float* a,
-                                                 const float* b, int lane,
-                                                 f32x4 c) {
-#pragma unroll
-  for (int k = 0; k < 16; k += 4)
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k + (lane >> 4)],
-                                             b[k + (lane >> 4)], c, 0, 0, 0);
-  return c;
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void gemm_any_kernel(GemmArgs g, int tiles_n) {
-  constexpr int BK = kAnyK<T>;
-  __shared__ __attribute__((aligned(16))) T as[64][BK + 16 / sizeof(T)];
-  __shared__ __attribute__((aligned(16))) T bs[64][BK + 16 / sizeof(T)];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int m0 = (int)(blockIdx.x / tiles_n) * 64;
-  const int n0 = (int)(blockIdx.x % tiles_n) * 64;
-  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
-  f32x4 acc[2][2] = {};
-  for (int k0 = 0; k0 < g.k; k0 += BK) {
-    __syncthreads();
-    any_stage<T>(g.a, m0, g.m, k0, g.k, as);
-    any_stage<T>(g.b, n0, g.n, k0, g.k, bs);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        acc[i][j] = mfma_row<T>(as[wm + i * 16 + (lane & 15)],
-                                bs[wn + j * 16 + (lane & 15)], lane, acc[i][j]);
-  }
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int col = n0 + wn + j * 16 + (lane & 15);
-    if (col >= g.n) continue;
-    float bias = 0.f;
-    if (g.bias) load_learned<1>(g.bias, g.bias_dt, col, 1, &bias);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = m0 + wm + i * 16 + (lane >> 4) * 4 + r;
-        if (row < g.m) finish<T>(g, row, col, acc[i][j][r], bias);
-      }
-  }
-}
-
-template <typename T>
-void gemm_any(const GemmArgs& g, hipStream_t st) {
-  const long tm = ((long)g.m + 63) / 64, tn = ((long)g.n + 63) / 64;
-  gemm_any_kernel<T><<<dim3((unsigned)(tm * tn)), dim3(256), 0, st>>>(g, (int)tn);
-}
-
-// ---------------------------------------------------------------------------
-// 16-bit products by tiles (gemm_tiles.h)
+// Products by tiles (gemm_tiles.h)
 // ---------------------------------------------------------------------------
 
 // Blocks go to the eight XCDs in turn, and each XCD has its own L2: give each
@@ -196,44 +61,64 @@ __device__ __forceinline__ void tile_of(int id, int tm, int tn, int& m, int& n) 
   n = id / rows;
 }
 
-// Eight neighbouring results of a row: bias, z, activation, residual.
-template <typename T>
-__device__ __forceinline__ void finish8(const GemmArgs& g, int row, int col,
-                                        float (&v)[8], const float* bias) {
+// N neighbouring results of a row: bias, z, activation, residual.
+template <typename T, int N>
+__device__ __forceinline__ void finish(const GemmArgs& g, int row, int col,
+                                       float (&v)[N], const float* bias) {
   const int left = g.n - col;
   if (row >= g.m || left <= 0) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] += bias[i];
-  if (g.z) store_vec<T>(static_cast<T*>(g.z) + (long)row * g.n + col, left, v);
+  for (int i = 0; i < N; ++i) v[i] += bias[i];
+  if (g.z)
+    store_some<T, N>(static_cast<T*>(g.z) + (long)row * g.n + col, left, v);
   if (g.act == Act::relu) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = act_value(v[i], Act::relu);
+    for (int i = 0; i < N; ++i) v[i] = act_value(v[i], Act::relu);
   } else if (g.act == Act::gelu) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = act_value(v[i], Act::gelu);
+    for (int i = 0; i < N; ++i) v[i] = act_value(v[i], Act::gelu);
   } else if (g.act == Act::silu) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = act_value(v[i], Act::silu);
+    for (int i = 0; i < N; ++i) v[i] = act_value(v[i], Act::silu);
   }
   if (g.res) {
-    float r[8];
-    load_vec<T>(static_cast<const T*>(g.res) + (long)row * g.res_ld + col, left,
-                0.f, r);
+    float r[N];
+    load_some<T, N>(static_cast<const T*>(g.res) + (long)row * g.res_ld + col,
+                    left, r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += r[i];
+    for (int i = 0; i < N; ++i) v[i] += r[i];
   }
-  store_vec<T>(static_cast<T*>(g.y) + (long)row * g.y_ld + col, left, v);
+  store_some<T, N>(static_cast<T*>(g.y) + (long)row * g.y_ld + col, left, v);
 }
 
-template <typename T>
+template <typename T, int F>
 __device__ __forceinline__ void leave_finished(const GemmArgs& g, char* lds,
-                                               f32x4 (&v)[4][4], int row0,
+                                               const f32x4 (*v)[4], int row0,
                                                int col0, int lane) {
   float bias[8] = {};
   const int col = col0 + (lane & 7) * 8;
   if (g.bias) load_learned<8>(g.bias, g.bias_dt, col, g.n - col, bias);
-  leave(lds, v, lane, [&](int row, int c, float (&out)[8]) {
-    finish8<T>(g, row0 + row, col0 + c, out, bias);
+  leave<F>(lds, v, lane, [&](int row, int c, float (&out)[8]) {
+    finish<T, 8>(g, row0 + row, col0 + c, out, bias);
+  });
+}
+
+// The same, or a slice's sums to `part`.
+template <typename T, int F>
+__device__ __forceinline__ void leave_block(const GemmArgs& g, char* lds,
+                                            const f32x4 (*v)[4], int row0,
+                                            int col0, int lane, int slice,
+                                            float* part) {
+  if (!part) {
+    leave_finished<T, F>(g, lds, v, row0, col0, lane);
+    return;
+  }
+  leave<F>(lds, v, lane, [&](int row, int col, float (&out)[8]) {
+    row += row0;
+    col += col0;
+    if (row < g.m && col < g.n)
+      store_some<float, 8>(part + ((long)slice * g.m + row) * g.n + col,
+                           g.n - col, out);
   });
 }
 
@@ -378,29 +263,33 @@ __global__ __launch_bounds__(512, 2) void gemm_256_kernel(GemmArgs g, int tm,
   __syncthreads();  // the tiles have been read
 #pragma unroll
   for (int h = 0; h < 2; ++h)
-    leave_finished<T>(g, lds + wave * kHalf, acc[h], m0 + h * 128 + wm,
+    leave_finished<T, 4>(g, lds + wave * kHalf, acc[h], m0 + h * 128 + wm,
                       n0 + (wave & 3) * 64, lane);
 }
 
-// 128 by 128 results, four waves of 64 by 64, two blocks a CU; the tiles of k
-// may be shared out over `slices` blocks, whose sums then go to `part` as
-// they are.  One barrier a tile: a wave that has passed it has its copies of
-// this tile and knows that the others are done with the one before.
+// 128 by 128 results, eight waves, one block a CU: four of 64 by 64 on the
+// first 32 k of a tile, four on the other 32.  LDS has four tiles, and a tile
+// is read into registers one step before it is multiplied, so that LDS reads
+// go on under the matrix instructions (read and multiplied in the same step a
+// tile took 0.74 us) and copies have three steps to land.  One barrier a
+// step: a wave that has passed it has its copies of tile t + 1 and knows that
+// all have read tile t, whose place tile t + 4 takes.  The tiles of k may be
+// shared out over `slices` blocks, whose sums then go to `part` as they are.
 template <typename T, bool AX, bool BX>
-__global__ __launch_bounds__(256, 2) void gemm_128_kernel(GemmArgs g, int tm,
+__global__ __launch_bounds__(512, 2) void gemm_128_kernel(GemmArgs g, int tm,
                                                           int tn, int slices,
                                                           float* part) {
-  __shared__ __attribute__((aligned(1024))) char lds[4 * kHalf];
+  __shared__ __attribute__((aligned(1024))) char lds[8 * kHalf];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slice = blockIdx.x / (tm * tn);
   int bm, bn;
   tile_of(blockIdx.x % (tm * tn), tm, tn, bm, bn);
   const int m0 = bm * 128, n0 = bn * 128;
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+  const int wk = wave >> 2, wm = (wave >> 1 & 1) * 64, wn = (wave & 1) * 64;
   const u32 lds0 = lds_address(lds);
-  Copier<AX, 4, false> ca;
-  Copier<BX, 4, false> cb;
+  Copier<AX, 8, false> ca;
+  Copier<BX, 8, false> cb;
   ca.start(g.a, m0, g.m, wave, lane);
   cb.start(g.b, n0, g.n, wave, lane);
   const int whole = g.k / kTileK;
@@ -409,53 +298,310 @@ __global__ __launch_bounds__(256, 2) void gemm_128_kernel(GemmArgs g, int tm,
   const int left = slice == slices - 1 ? g.k % kTileK : 0;
 
   f32x4 acc[4][4] = {};
-  auto copy = [&](int t, int buf) {
-    ca.half(t, 0, lds0 + buf * (2 * kHalf));
-    cb.half(t, 0, lds0 + buf * (2 * kHalf) + kHalf);
+  auto copy = [&](int t) {
+    const u32 at = lds0 + ((t - from) & 3) * (2 * kHalf);
+    ca.half(t, 0, at);
+    cb.half(t, 0, at + kHalf);
   };
-  auto compute = [&](const char* buf) {
+  struct Fragments {
+    s16x8 a[4], b[4];
+  };
+  auto read = [&](const char* buf, Fragments& f) {
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      s16x8 fa[4], fb[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        fa[i] = fragment<AX>(buf, wm + i * 16, kk, lane);
-        fb[i] = fragment<BX>(buf + kHalf, wn + i * 16, kk, lane);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mfma<T>(fb[j], fa[i], acc[i][j]);
+    for (int i = 0; i < 4; ++i) {
+      f.a[i] = fragment<AX>(buf, wm + i * 16, wk, lane);
+      f.b[i] = fragment<BX>(buf + kHalf, wn + i * 16, wk, lane);
     }
   };
-  if (from < to) copy(from, 0);
-  for (int t = from; t < to; ++t) {
-    const int buf = (t - from) & 1;
-    wait_copies<0>();
+  auto multiply = [&](const Fragments& f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        acc[i][j] = mfma<T>(f.b[j], f.a[i], acc[i][j]);
+  };
+  Fragments f0, f1;
+  if (from < to) {
+    for (int t = from; t < min(from + 4, to); ++t) copy(t);
+    // four copies a lane for each tile
+    if (from + 4 <= to)
+      wait_copies<12>();
+    else
+      wait_copies<0>();
     block_barrier();
-    if (t + 1 < to) copy(t + 1, buf ^ 1);
-    compute(lds + buf * (2 * kHalf));
+    read(lds, f0);
   }
+  auto step = [&](int t, const Fragments& now, Fragments& next) {
+    if (t + 1 < to) {
+      if (t + 3 < to)
+        wait_copies<8>();
+      else
+        wait_copies<0>();
+      block_barrier();
+      if (t + 4 < to) copy(t + 4);
+      read(lds + ((t + 1 - from) & 3) * (2 * kHalf), next);
+    }
+    multiply(now);
+  };
+  for (int t = from; t < to; t += 2) {
+    step(t, f0, f1);
+    if (t + 1 < to) step(t + 1, f1, f0);
+  }
+  __syncthreads();
   if (left) {
-    __syncthreads();
     ca.rest(whole, 0, lds, left, lane);
     cb.rest(whole, 0, lds + kHalf, left, lane);
     __syncthreads();
-    compute(lds);
+    read(lds, f0);
+    multiply(f0);
+    __syncthreads();
   }
+  // the two halves of k: each wave finishes 32 of its 64 rows
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<f32x4*>(lds + wave * 8192 + (i * 4 + j) * 1024 +
+                                lane * 16) = wk ? acc[i][j] : acc[2 + i][j];
   __syncthreads();
-  if (!part) {
-    leave_finished<T>(g, lds + wave * kHalf, acc, m0 + wm, n0 + wn, lane);
+  f32x4 out[2][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      out[i][j] = (wk ? acc[2 + i][j] : acc[i][j]) +
+                  *reinterpret_cast<const f32x4*>(
+                      lds + (wave ^ 4) * 8192 + (i * 4 + j) * 1024 + lane * 16);
+  __syncthreads();
+  leave_block<T, 2>(g, lds + wave * 8192, out, m0 + wm + wk * 32, n0 + wn, lane,
+                 slice, part);
+}
+
+// 128 by 128 results of floats (gemm_tiles.h), tiles of 32 k.  Waves 4-7 read
+// floats three tiles ahead, cut them into planes and write those to LDS; waves
+// 0-3, one on each SIMD beside one of the others, multiply 64 by 64 each.  So
+// the cutting (900 cycles a tile) goes on under the matrix instructions (1536);
+// with both done by all eight waves in turn a tile took 1.6 us.
+template <bool AX, bool BX>
+__global__ __launch_bounds__(512, 2) void gemm_float_kernel(GemmArgs g, int tm,
+                                                            int tn, int slices,
+                                                            float* part) {
+  __shared__ __attribute__((aligned(1024))) char lds[12 * kPlane];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int slice = blockIdx.x / (tm * tn);
+  int bm, bn;
+  tile_of(blockIdx.x % (tm * tn), tm, tn, bm, bn);
+  const int m0 = bm * 128, n0 = bn * 128;
+  const int all = (g.k + kFloatK - 1) / kFloatK;
+  const int per = (all + slices - 1) / slices;
+  const int from = min(slice * per, all), to = min(from + per, all);
+  // Both halves of the waves pass one barrier a tile, and none elsewhere.
+  auto meet = [] {  // (not __syncthreads: loads stay in flight)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    block_barrier();
+  };
+  if (wave >= 4) {
+    const int tid = threadIdx.x - 256;
+    FloatStager<AX> sa[2];
+    FloatStager<BX> sb[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      sa[i].start(g.a, m0, g.m, tid + i * 256);
+      sb[i].start(g.b, n0, g.n, tid + i * 256);
+    }
+    struct Raw {
+      float a[2][8], b[2][8];
+    };
+    auto load = [&](int t, Raw& r) {
+      if (t >= to) return;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        sa[i].load(t, g.k - t * kFloatK, r.a[i]);
+        sb[i].load(t, g.k - t * kFloatK, r.b[i]);
+      }
+    };
+    // writes tile t, orders tile t + 3 in its place
+    auto step = [&](int t, Raw& r) {
+      if (t >= to) return;
+      char* buf = lds + ((t - from) & 1) * (6 * kPlane);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        sa[i].store(buf, r.a[i]);
+        sb[i].store(buf + 3 * kPlane, r.b[i]);
+      }
+      load(t + 3, r);
+      // tile t is there; and tile t - 1 has been read, whose place t + 1 takes
+      meet();
+    };
+    Raw r0, r1, r2;
+    load(from, r0);
+    load(from + 1, r1);
+    load(from + 2, r2);
+    for (int t = from; t < to; t += 3) {
+      step(t, r0);
+      step(t + 1, r1);
+      step(t + 2, r2);
+    }
     return;
   }
-  leave(lds + wave * kHalf, acc, lane, [&](int row, int col, float (&out)[8]) {
-    row += m0 + wm;
-    col += n0 + wn;
-    if (row >= g.m) return;
-    float* p = part + ((long)slice * g.m + row) * g.n + col;
-    store_vec<float>(p, g.n - col, out);
-    store_vec<float>(p + 4, g.n - col - 4, out + 4);
-  });
+  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+  f32x4 acc[4][4] = {};
+  for (int t = from; t < to; ++t) {
+    meet();
+    const char* buf = lds + ((t - from) & 1) * (6 * kPlane);
+    s16x8 fa[3][4], fb[3][4];
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        fa[q][i] = float_fragment<AX>(buf + q * kPlane, wm + i * 16, lane);
+        fb[q][i] = float_fragment<BX>(buf + (3 + q) * kPlane, wn + i * 16, lane);
+      }
+    // in the order in which the planes arrive
+#pragma unroll
+    for (int sum = 0; sum < 3; ++sum)
+#pragma unroll
+      for (int q = 0; q <= sum; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc[i][j] = mfma<bf16_t>(fb[sum - q][j], fa[q][i], acc[i][j]);
+  }
+  // The producers wrote their last tile before the last barrier; but the other
+  // waves may still be reading it, so each wave leaves through the half of LDS
+  // that the last tile is not in, 12 KB a wave: 48 rows, then 16.
+  char* free = lds + ((to - from) & 1) * (6 * kPlane) + wave * 12288;
+  leave_block<float, 3>(g, free, acc, m0 + wm, n0 + wn, lane, slice, part);
+  leave_block<float, 1>(g, free, acc + 3, m0 + wm + 48, n0 + wn, lane, slice,
+                        part);
+}
+
+// Few rows of A (16 F), both operands along: bound by reading B once.  A block
+// has 16 W rows of B; its eight waves share out k and add up through LDS.  B
+// goes straight into registers, a whole 128-byte line a row at a time, and A
+// comes from the caches, two batches of lines in flight a wave; nothing asks
+// for alignment.  Where there are few blocks and much k, `slices` of them share
+// a row's k as above.
+//
+// A is read once for every 16 W rows of B, which limits how many rows pay: with
+// 134 MB of 16-bit B, 8, 16, 32 and 48 rows took 34, 39, 50 and 66 us for W = 1
+// and 34, 37, 40 and 50 for W = 2 against 40 of gemm_128_kernel; with 34 MB 11,
+// 12, 16 and 21 against 17; with 8 MB 6, 7, 7 and 9 against 14.
+template <typename T, int F, int W>
+__global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g, int slices,
+                                                        float* part) {
+  constexpr int VEC = 16 / sizeof(T);    // a lane's elements of a load
+  constexpr int UNIT = 128 / sizeof(T);  // k of a line; a lane has two loads
+  constexpr int BATCH = F == 1 ? (W == 1 ? 4 : 2) : F == 2 && W == 1 ? 2 : 1;
+  typedef T V __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
+  __shared__ f32x4 sums[8][F * W][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int blocks = (g.n + 16 * W - 1) / (16 * W);
+  const int slice = blockIdx.x / blocks;
+  const int n0 = (blockIdx.x % blocks) * (16 * W);
+  const int units = (g.k + UNIT - 1) / UNIT;
+  const int per = (units + slices - 1) / slices;
+  const int from = slice * per, to = min(from + per, units);
+  const int k0 = (lane >> 4) * 2 * VEC;
+  // (rows behind the last one repeat it: their results are not stored)
+  const T *a[F], *b[W];
+#pragma unroll
+  for (int w = 0; w < W; ++w)
+    b[w] = static_cast<const T*>(g.b.p) +
+           (long)min(n0 + w * 16 + (lane & 15), g.n - 1) * g.b.ld + k0;
+#pragma unroll
+  for (int f = 0; f < F; ++f)
+    a[f] = static_cast<const T*>(g.a.p) +
+           (long)min(f * 16 + (lane & 15), g.m - 1) * g.a.ld + k0;
+
+  struct Lines {
+    V b[BATCH][W][2], a[BATCH][F][2];
+  };
+  auto fetch = [&](const T* p, int k, bool in, V (&v)[2]) {
+    const int left = in ? g.k - k - k0 : 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (left >= (h + 1) * VEC) {
+        v[h] = *reinterpret_cast<const V*>(p + k + h * VEC);
+      } else {
+        v[h] = V{};
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (h * VEC + i < left) v[h][i] = p[k + h * VEC + i];
+      }
+    }
+  };
+  // unit u and the BATCH - 1 that this wave has behind it
+  auto load = [&](int u, Lines& l) {
+#pragma unroll
+    for (int q = 0; q < BATCH; ++q) {
+      const int k = (u + q * 8) * UNIT;
+      const bool in = u + q * 8 < to;
+#pragma unroll
+      for (int w = 0; w < W; ++w) fetch(b[w], k, in, l.b[q][w]);
+#pragma unroll
+      for (int f = 0; f < F; ++f) fetch(a[f], k, in, l.a[q][f]);
+    }
+  };
+  f32x4 acc[F][W] = {};
+  auto multiply = [&](const Lines& l) {
+#pragma unroll
+    for (int q = 0; q < BATCH; ++q)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int f = 0; f < F; ++f)
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            if constexpr (__is_same(T, float)) {
+              // any order of k does, if it is both operands'
+#pragma unroll
+              for (int i = 0; i < VEC; ++i)
+                acc[f][w] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                    l.b[q][w][h][i], l.a[q][f][h][i], acc[f][w], 0, 0, 0);
+            } else {
+              acc[f][w] = mfma<T>(__builtin_bit_cast(s16x8, l.b[q][w][h]),
+                                  __builtin_bit_cast(s16x8, l.a[q][f][h]),
+                                  acc[f][w]);
+            }
+          }
+  };
+  constexpr int STRIDE = 8 * BATCH;
+  Lines l0, l1;
+  int u = from + wave;
+  if (u < to) load(u, l0);
+  for (; u < to; u += 2 * STRIDE) {
+    if (u + STRIDE < to) load(u + STRIDE, l1);
+    multiply(l0);
+    if (u + STRIDE < to) {
+      if (u + 2 * STRIDE < to) load(u + 2 * STRIDE, l0);
+      multiply(l1);
+    }
+  }
+#pragma unroll
+  for (int f = 0; f < F; ++f)
+#pragma unroll
+    for (int w = 0; w < W; ++w) sums[wave][f * W + w][lane] = acc[f][w];
+  __syncthreads();
+  // 16 by 16 results a wave, four neighbours a lane
+  for (int i = wave; i < F * W; i += 8) {
+    f32x4 t = sums[0][i][lane];
+#pragma unroll
+    for (int s = 1; s < 8; ++s) t += sums[s][i][lane];
+    const int row = i / W * 16 + (lane & 15);
+    const int col = n0 + i % W * 16 + (lane >> 4) * 4;
+    float v[4] = {t[0], t[1], t[2], t[3]}, bias[4] = {};
+    if (part) {
+      if (row < g.m && col < g.n)
+        store_some<float, 4>(part + ((long)slice * g.m + row) * g.n + col,
+                             g.n - col, v);
+      continue;
+    }
+    if (g.bias) load_learned<4>(g.bias, g.bias_dt, col, g.n - col, bias);
+    finish<T, 4>(g, row, col, v, bias);
+  }
 }
 
 // The slices' sums, in order, and what follows the product.
@@ -475,43 +621,100 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs g, int slices,
       for (int q = 0; q < 8; ++q) v[q] += u[q];
     }
     if (g.bias) load_learned<8>(g.bias, g.bias_dt, col, g.n - col, bias);
-    finish8<T>(g, row, col, v, bias);
+    finish<T, 8>(g, row, col, v, bias);
   }
 }
 
-// How a 16-bit product is cut up.
+}  // namespace
+
+// Whether gemm_rows_kernel takes a product of operands along (its figures).
+bool gemm_few_rows(long m, long n, long k, Dt dt) {
+  return m <= 32 || (m <= 64 && n * k * dt_size(dt) <= (16L << 20));
+}
+
+namespace {
+
+// How a product is cut up.  Both kernels have one block a CU, so time goes by
+// rounds of 256 blocks.  In units of a 128-tile's 64 k (0.35 us): a 256-tile's
+// take 2.6, what a block does before and behind its loop 6 and 12, and the
+// joining kernel its 8 bytes for each partial sum, at 4 TB/s, and its launch.
 struct Plan {
-  int tile;    // 256 or 128
-  int slices;  // of k, for 128
+  int tile;    // 256 or 128; 32 or 16 for gemm_rows_kernel
+  int slices;  // of k, not for 256
 };
 
-Plan plan_for(long m, long n, long k) {
+Plan plan_for(long m, long n, long k, Dt dt, bool along) {
   if (m < 1 || n < 1) return {128, 1};  // nothing will be launched
-  const long big = ((m + 255) / 256) * ((n + 255) / 256);
-  if (big >= 192) return {256, 1};
-  const long small = ((m + 127) / 128) * ((n + 127) / 128);
-  long slices = (512 + small - 1) / small;  // two blocks a CU
-  const long most = k / (kTileK * 4);       // four tiles a slice at least
-  if (slices > most) slices = most;
-  return {128, (int)(slices < 1 ? 1 : slices)};
+  if (along && gemm_few_rows(m, n, k, dt)) {
+    // 16 rows of B a block, or 32 where A would be read too often
+    const bool wide = m <= 32 && n * k * dt_size(dt) > (48L << 20);
+    const long blocks = wide ? (n + 31) / 32 : (n + 15) / 16;
+    const long lines = k * dt_size(dt) / 128;
+    long s = 512 / blocks;  // two blocks a CU, eight lines a wave at least
+    if (s > lines / 64) s = lines / 64;
+    return {wide ? 32 : 16, (int)(s < 1 ? 1 : s > 32 ? 32 : s)};
+  }
+  auto count = [&](long t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
+  auto rounds = [](long blocks) { return (double)((blocks + 255) / 256); };
+  const bool floats = dt == Dt::f32;
+  const long tile_k = floats ? kFloatK : kTileK;
+  const long tiles = (k + tile_k - 1) / tile_k;
+  const double unit = floats ? 2.4 : 1;  // of a 128-tile's k
+  const long small = count(128);
+  Plan best = {256, 1};
+  double least = floats ? 1e30 : rounds(count(256)) * (2.6 * tiles + 12);
+  for (int s = 1; s <= 32 && (s == 1 || tiles / s >= 4); ++s) {
+    double cost = rounds(small * s) * ((tiles + s - 1) / s * unit + 6);
+    if (s > 1) cost += 10 + s * (double)m * n * 8 / 1.4e6;
+    if (cost < least) {
+      least = cost;
+      best = {128, s};
+    }
+  }
+  return best;
+}
+
+template <typename O>
+void join_slices(const GemmArgs& g, const Plan& p, hipStream_t st) {
+  const long blocks = ((long)g.m * ((g.n + 7) / 8) + 255) / 256;
+  gemm_join_kernel<O><<<dim3((unsigned)(blocks < 4096 ? blocks : 4096)),
+                        dim3(256), 0, st>>>(g, p.slices, g.work);
 }
 
 template <typename T, bool AX, bool BX>
 void gemm_tiles_t(const GemmArgs& g, hipStream_t st) {
-  const Plan p = plan_for(g.m, g.n, g.k);
+  const Plan p = plan_for(g.m, g.n, g.k, g.dt, !g.a.across && !g.b.across);
   const int tm = (g.m + p.tile - 1) / p.tile, tn = (g.n + p.tile - 1) / p.tile;
-  if (p.tile == 256) {
-    gemm_256_kernel<T, AX, BX><<<dim3(tm * tn), dim3(512), 0, st>>>(g, tm, tn);
-    return;
-  }
   float* part = p.slices > 1 ? g.work : nullptr;
-  gemm_128_kernel<T, AX, BX><<<dim3(tm * tn * p.slices), dim3(256), 0, st>>>(
-      g, tm, tn, p.slices, part);
-  if (part) {
-    const long blocks = ((long)g.m * ((g.n + 7) / 8) + 255) / 256;
-    gemm_join_kernel<T><<<dim3((unsigned)(blocks < 4096 ? blocks : 4096)),
-                          dim3(256), 0, st>>>(g, p.slices, part);
+  const dim3 grid(tm * tn * p.slices);
+  if constexpr (!AX && !BX) {
+    if (p.tile < 128) {
+      const dim3 grid(tn * p.slices);
+      auto start = [&](auto f, auto w) {
+        gemm_rows_kernel<T, decltype(f)::value, decltype(w)::value>
+            <<<grid, dim3(512), 0, st>>>(g, p.slices, part);
+      };
+      using std::integral_constant;
+      const integral_constant<int, 1> one;
+      const integral_constant<int, 2> two;
+      const integral_constant<int, 4> four;
+      if (p.tile == 32)
+        g.m <= 16 ? start(one, two) : start(two, two);
+      else
+        g.m <= 16 ? start(one, one) : g.m <= 32 ? start(two, one) : start(four, one);
+      if (part) join_slices<T>(g, p, st);
+      return;
+    }
   }
+  if constexpr (__is_same(T, float))
+    gemm_float_kernel<AX, BX><<<grid, dim3(512), 0, st>>>(g, tm, tn, p.slices,
+                                                          part);
+  else if (p.tile == 256)
+    gemm_256_kernel<T, AX, BX><<<grid, dim3(512), 0, st>>>(g, tm, tn);
+  else
+    gemm_128_kernel<T, AX, BX><<<grid, dim3(512), 0, st>>>(g, tm, tn, p.slices,
+                                                           part);
+  if (part) join_slices<T>(g, p, st);
 }
 
 template <typename T>
@@ -595,16 +798,15 @@ __global__ __launch_bounds__(256) void column_join_kernel(
 void gemm_fused(const GemmArgs& g, hipStream_t st) {
   if (g.m == 0 || g.n == 0) return;
   if (g.dt == Dt::f32)
-    gemm_any<float>(g, st);
+    gemm_tiles<float>(g, st);
   else if (g.dt == Dt::bf16)
     gemm_tiles<bf16_t>(g, st);
   else
     gemm_tiles<f16_t>(g, st);
 }
 
-long gemm_work_floats(long m, long n, long k, Dt dt) {
-  if (dt == Dt::f32) return 0;
-  const Plan p = plan_for(m, n, k);
+long gemm_work_floats(long m, long n, long k, Dt dt, bool along) {
+  const Plan p = plan_for(m, n, k, dt, along);
   return p.slices > 1 ? p.slices * m * n : 0;
 }
 

@@ -386,7 +386,9 @@ def run_linear(device, dtype, m, k, n, act=None, residual=False, bias=True,
 LINEAR_SHAPES = [(1, 1, 1), (1, 64, 100), (2, 7, 3), (5, 129, 65),
                  (16, 256, 64), (17, 72, 40), (64, 64, 64), (65, 96, 130),
                  (128, 128, 128), (100, 333, 71), (129, 200, 257),
-                 (256, 64, 256), (300, 520, 264)]
+                 (256, 64, 256), (300, 520, 264), (64, 66, 31), (33, 130, 47),
+                 (1, 9001, 20), (40, 20000, 17), (70, 2600, 150),
+                 (257, 1300, 40)]
 
 
 @on_devices
