@@ -12,7 +12,6 @@ import math
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -20,32 +19,6 @@ __all__ = ["fused_linear", "FusedLinear"]
 
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 _ACTS = {None: 0, "relu": 1, "gelu": 2, "silu": 3}
-
-
-class _FusedLinearFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, act, residual):
-        # relu's slope can be read off its own output, unless a residual was
-        # added to that
-        from_y = act == 1 and residual is None
-        y, z = ops.hip_ext().linear_fwd(x, weight, bias, act, residual,
-                                        act != 0 and not from_y)
-        ctx.act = act
-        ctx.bias_type = x.dtype if bias is None else bias.dtype
-        ctx.save_for_backward(x, weight, y if from_y else z)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, z = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx = dw = db = None
-        if any(need[:3]):
-            dx, dw, db = ops.hip_ext().linear_bwd(
-                dy, x, weight, z, ctx.act, need[0], need[1], need[2],
-                ctx.bias_type)
-        return dx, dw, db, None, dy if need[4] else None
 
 
 def _check(x, weight, bias, residual):
@@ -106,11 +79,7 @@ def fused_linear(x, weight, bias=None, activation=None, residual=None):
     act = _ACTS[activation]
     if not x.is_cuda:
         return _eager(x, weight, bias, act, residual)
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad
-            for t in (x, weight, bias, residual)):
-        return _FusedLinearFn.apply(x, weight, bias, act, residual)
-    return ops.hip_ext().linear_fwd(x, weight, bias, act, residual, False)[0]
+    return ops.hip_ext().linear(x, weight, bias, act, residual)
 
 
 class FusedLinear(nn.Module):

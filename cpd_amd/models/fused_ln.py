@@ -13,35 +13,12 @@ take raises, and a missing HIP extension raises.
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from .. import ops
 
 __all__ = ["fused_layer_norm", "FusedLayerNorm"]
 
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
-
-
-class _FusedLNFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps, residual):
-        y, s, stats = ops.hip_ext().norm_fwd(x, weight, bias, eps, residual)
-        ctx.set_materialize_grads(False)
-        ctx.bias_type = x.dtype if bias is None else bias.dtype
-        ctx.save_for_backward(x if residual is None else s, weight, stats)
-        return y if residual is None else (y, s)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, ds=None):
-        if dy is None and ds is None:
-            return None, None, None, None, None
-        s, weight, stats = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx, dw, db = ops.hip_ext().norm_bwd(s, dy, ds, weight, stats, need[1],
-                                            need[2], ctx.bias_type)
-        return (dx if need[0] else None, dw, db, None,
-                dx if need[4] else None)
 
 
 def _check(x, weight, bias, residual):
@@ -116,12 +93,8 @@ def fused_layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
     """
     if not x.is_cuda:
         return _eager(x, weight, bias, eps, residual)
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad
-            for t in (x, weight, bias, residual)):
-        return _FusedLNFn.apply(x, weight, bias, eps, residual)
-    y, s, _ = ops.hip_ext().norm_fwd(x, weight, bias, eps, residual)
-    return y if residual is None else (y, s)
+    out = ops.hip_ext().layer_norm(x, weight, bias, eps, residual)
+    return out[0] if residual is None else tuple(out)
 
 
 class FusedLayerNorm(nn.Module):

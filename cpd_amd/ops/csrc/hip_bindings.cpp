@@ -496,16 +496,157 @@ std::vector<Tensor> linear_bwd(const Tensor& dy, const Tensor& x,
   return {dx, dw, db};
 }
 
+// ---------------------------------------------------------------------------
+// The operators with their gradients.  The graph's nodes are C++: a backward
+// pass through Python's own function class costs about 50 us of waiting for
+// the interpreter, more than most of these kernels take.
+// ---------------------------------------------------------------------------
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool wants_grad(const OptTensor& t) {
+  return t.has_value() && t->defined() && t->requires_grad();
+}
+
+bool present(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+OptTensor some(const Tensor& t) {
+  return t.defined() ? OptTensor(t) : std::nullopt;
+}
+
+// (an edge for every tensor that forward was given, in its order)
+bool needs(const AutogradContext* ctx, const char* name) {
+  const auto edge = ctx->saved_data.at(name).toInt();
+  return edge >= 0 && ctx->needs_input_grad(edge);
+}
+void name_edges(AutogradContext* ctx,
+                std::initializer_list<std::pair<const char*, bool>> inputs) {
+  int64_t edge = 0;
+  for (const auto& in : inputs) ctx->saved_data[in.first] = in.second ? edge++ : -1;
+}
+
+void check_once(const char* what) {
+  // gradients are asked for with their own graph only to differentiate again
+  TORCH_CHECK(!at::GradMode::is_enabled(), what,
+              " cannot be differentiated twice (create_graph=True)");
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x,
+                               const OptTensor& weight, const OptTensor& bias,
+                               double eps, const OptTensor& residual) {
+    auto out = norm_fwd(x, weight, bias, eps, residual);
+    ctx->set_materialize_grads(false);
+    name_edges(ctx, {{"x", true}, {"weight", present(weight)},
+                     {"bias", present(bias)}, {"residual", present(residual)}});
+    ctx->saved_data["type"] = bias ? bias->scalar_type() : x.scalar_type();
+    ctx->save_for_backward({residual ? out[1] : x, weight.value_or(Tensor()),
+                            out[2]});
+    if (residual) return {out[0], out[1]};
+    return {out[0]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_once("layer norm");
+    const Tensor ds = g.size() > 1 ? g[1] : Tensor();
+    if (!g[0].defined() && !ds.defined()) return variable_list(5);
+    const auto saved = ctx->get_saved_variables();
+    auto d = norm_bwd(saved[0], some(g[0]), some(ds), some(saved[1]), saved[2],
+                      needs(ctx, "weight"), needs(ctx, "bias"),
+                      ctx->saved_data["type"].toScalarType());
+    return {needs(ctx, "x") ? d[0] : Tensor(), d[1], d[2], Tensor(),
+            needs(ctx, "residual") ? d[0] : Tensor()};
+  }
+};
+
+std::vector<Tensor> layer_norm(const Tensor& x, const OptTensor& weight,
+                               const OptTensor& bias, double eps,
+                               const OptTensor& residual) {
+  if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) ||
+                                     wants_grad(bias) || wants_grad(residual)))
+    return LayerNorm::apply(x, weight, bias, eps, residual);
+  auto out = norm_fwd(x, weight, bias, eps, residual);
+  out.resize(residual ? 2 : 1);
+  return out;
+}
+
+struct Linear : torch::autograd::Function<Linear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x,
+                        const Tensor& weight, const OptTensor& bias, int64_t act,
+                        const OptTensor& residual) {
+    // relu's slope can be read off its own output, unless a residual was added
+    // to that
+    const bool from_y = act_of(act) == cpd::Act::relu && !residual;
+    auto out = linear_fwd(x, weight, bias, act, residual, act != 0 && !from_y);
+    ctx->set_materialize_grads(false);
+    name_edges(ctx, {{"x", true}, {"weight", true}, {"bias", present(bias)},
+                     {"residual", present(residual)}});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["type"] = bias ? bias->scalar_type() : x.scalar_type();
+    ctx->save_for_backward({x, weight, from_y ? out[0] : out[1]});
+    return out[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_once("linear");
+    const Tensor dy = g[0];
+    if (!dy.defined()) return variable_list(5);
+    const bool x = needs(ctx, "x"), w = needs(ctx, "weight"), b = needs(ctx, "bias");
+    std::vector<Tensor> d(3);
+    if (x || w || b) {
+      const auto saved = ctx->get_saved_variables();
+      d = linear_bwd(dy, saved[0], saved[1], some(saved[2]),
+                     ctx->saved_data["act"].toInt(), x, w, b,
+                     ctx->saved_data["type"].toScalarType());
+    }
+    return {d[0], d[1], d[2], Tensor(), needs(ctx, "residual") ? dy : Tensor()};
+  }
+};
+
+Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias,
+              int64_t act, const OptTensor& residual) {
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || weight.requires_grad() || wants_grad(bias) ||
+       wants_grad(residual)))
+    return Linear::apply(x, weight, bias, act, residual);
+  return linear_fwd(x, weight, bias, act, residual, false)[0];
+}
+
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x,
+                               const Tensor& targets, int64_t top, int64_t ignore) {
+    auto out = logprob_fwd(x, targets, top, ignore);
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["ignore"] = ignore;
+    ctx->save_for_backward({x, targets, out[2], out[1]});
+    if (!top) return {out[0], out[1]};
+    ctx->mark_non_differentiable({out[3], out[4]});
+    return {out[0], out[1], out[3], out[4]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_once("token log probabilities");
+    if (!g[0].defined() && !g[1].defined()) return variable_list(4);
+    const auto saved = ctx->get_saved_variables();
+    return {logprob_bwd(saved[0], saved[1], saved[2], saved[3], some(g[0]),
+                        some(g[1]), ctx->saved_data["ignore"].toInt()),
+            Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// logprobs, entropy, and with top > 0 ids and log probabilities
+std::vector<Tensor> token_logprobs(const Tensor& x, const Tensor& targets,
+                                   int64_t top, int64_t ignore) {
+  if (at::GradMode::is_enabled() && x.requires_grad())
+    return TokenLogprobs::apply(x, targets, top, ignore);
+  auto out = logprob_fwd(x, targets, top, ignore);
+  if (!top) return {out[0], out[1]};
+  return {out[0], out[1], out[3], out[4]};
+}
+
 }  // namespace
 
 void cpd_register_fused(pybind11::module_& m) {
-  m.def("norm_fwd", &norm_fwd,
-        "layer norm (+residual): returns (y, s, stats)");
-  m.def("norm_bwd", &norm_bwd,
-        "layer norm backward: returns (dx, dweight, dbias)");
-  m.def("logprob_fwd", &logprob_fwd,
-        "returns (logprobs, entropy, stats, top_ids, top_logprobs)");
-  m.def("logprob_bwd", &logprob_bwd, "gradient of the logits");
-  m.def("linear_fwd", &linear_fwd, "act(x W^T + b) + residual: (y, z)");
-  m.def("linear_bwd", &linear_bwd, "returns (dx, dweight, dbias)");
+  m.def("layer_norm", &layer_norm, "layer norm (+residual): [y] or [y, s]");
+  m.def("linear", &linear, "act(x W^T + bias) + residual");
+  m.def("token_logprobs", &token_logprobs,
+        "[logprobs, entropy] or [logprobs, entropy, top_ids, top_logprobs]");
 }

@@ -10,7 +10,6 @@ are the only path.
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -25,30 +24,6 @@ class TokenLogprobs(NamedTuple):
     entropy: torch.Tensor                   # [...] float32, in nats
     top_ids: Optional[torch.Tensor]         # [..., top_k] int64
     top_logprobs: Optional[torch.Tensor]    # [..., top_k] float32
-
-
-class _TokenLogprobsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, targets, top_k, ignore_index):
-        lp, ent, stats, ids, tops = ops.hip_ext().logprob_fwd(
-            logits, targets, top_k, ignore_index)
-        ctx.set_materialize_grads(False)
-        ctx.ignore_index = ignore_index
-        ctx.save_for_backward(logits, targets, stats, ent)
-        if not top_k:
-            return lp, ent, None, None
-        ctx.mark_non_differentiable(ids, tops)
-        return lp, ent, ids, tops
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, glp, gent, *_):
-        if glp is None and gent is None:
-            return None, None, None, None
-        logits, targets, stats, ent = ctx.saved_tensors
-        return ops.hip_ext().logprob_bwd(logits, targets, stats, ent, glp,
-                                         gent, ctx.ignore_index), \
-            None, None, None
 
 
 def _check(logits, targets, top_k):
@@ -124,9 +99,5 @@ def token_logprobs(logits, targets, top_k=0, ignore_index=-100):
     """
     if not logits.is_cuda:
         return _eager(logits, targets, top_k, ignore_index)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return TokenLogprobs(*_TokenLogprobsFn.apply(logits, targets, top_k,
-                                                     ignore_index))
-    lp, ent, _, ids, tops = ops.hip_ext().logprob_fwd(logits, targets, top_k,
-                                                      ignore_index)
-    return TokenLogprobs(lp, ent, ids, tops)
+    out = ops.hip_ext().token_logprobs(logits, targets, top_k, ignore_index)
+    return TokenLogprobs(*out) if top_k else TokenLogprobs(*out, None, None)

@@ -951,6 +951,19 @@ def step_of(m, x, t):
 
 
 @pytest.mark.gpu
+def test_gpu_not_twice_differentiable():
+    """Asked for a graph of the gradient, the kernels say no instead of
+    leaving a part of it out."""
+    x = torch.randn(4, 16, device="cuda", requires_grad=True)
+    w = torch.randn(8, 16, device="cuda")
+    t = torch.zeros(4, dtype=torch.int64, device="cuda")
+    for y in (fused_layer_norm(x), fused_linear(x, w, activation="silu"),
+              token_logprobs(x, t).logprobs):
+        with pytest.raises(RuntimeError, match="twice"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+@pytest.mark.gpu
 @on_types
 def test_gpu_twice_the_same(dtype):
     torch.manual_seed(3)
