@@ -107,33 +107,79 @@ __device__ __forceinline__ void store_as(void* p, Dt dt, long at, float v) {
     static_cast<f16_t*>(p)[at] = (f16_t)v;
 }
 
-// Sum over groups of `W` neighbouring lanes (a power of two up to 64); every
-// lane of a group gets it.
-template <int W>
-__device__ __forceinline__ float group_sum(float v) {
+// 16 bytes as they are; elements at or behind `left` are zero.
+template <typename T>
+__device__ __forceinline__ typename Vec16<T>::type load_raw(const T* p,
+                                                            int left) {
+  typedef typename Vec16<T>::type V;
+  if (left >= Vec16<T>::N) return *reinterpret_cast<const V*>(p);
+  V v = {};
 #pragma unroll
-  for (int d = W / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+  for (int i = 0; i < Vec16<T>::N; ++i)
+    if (i < left) v[i] = p[i];
   return v;
 }
 
-// Sum over the TPR threads that share a row: within a wave by lanes, over
-// waves through `smem` (two floats a wave; `turn` alternates 0/1 from call to
-// call, so that one barrier a call is enough).
+// v of the lane `N` places on within its 16 lanes, round and round.
+template <int N>
+__device__ __forceinline__ float rotate16(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(
+      0, __float_as_int(v), 0x120 + N, 0xf, 0xf, true));
+}
+
+__device__ __forceinline__ float lane_value(float v, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+
+// Sum over groups of `W` = 16 or 64 neighbouring lanes, all of them active;
+// every lane of a group gets it.  (Rotations within the instruction: a shuffle
+// through LDS takes ten times as long.)
+template <int W>
+__device__ __forceinline__ float group_sum(float v) {
+  static_assert(W == 16 || W == 64, "a quarter of a wave, or a wave");
+  v += rotate16<8>(v);
+  v += rotate16<4>(v);
+  v += rotate16<2>(v);
+  v += rotate16<1>(v);
+  if constexpr (W == 64)
+    v = (lane_value(v, 0) + lane_value(v, 16)) +
+        (lane_value(v, 32) + lane_value(v, 48));
+  return v;
+}
+
+// Sums of two values over the TPR threads that share a row: within a wave by
+// lanes, over waves through `smem` (4 TPR/64 floats).  `turn` alternates 0/1
+// from call to call, so that one barrier a call is enough.
+template <int TPR>
+__device__ __forceinline__ void row_sums(float& a, float& b, float* smem,
+                                         int turn) {
+  constexpr int WAVES = TPR / 64;
+  if constexpr (TPR <= 64) {
+    a = group_sum<TPR>(a);
+    b = group_sum<TPR>(b);
+  } else {
+    a = group_sum<64>(a);
+    b = group_sum<64>(b);
+    float* s = smem + turn * 2 * WAVES;
+    if ((threadIdx.x & 63) == 0) {
+      s[threadIdx.x >> 6] = a;
+      s[WAVES + (threadIdx.x >> 6)] = b;
+    }
+    __syncthreads();
+    a = b = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      a += s[w];
+      b += s[WAVES + w];
+    }
+  }
+}
+
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* smem, int turn) {
-  if constexpr (TPR <= 64) {
-    return group_sum<TPR>(v);
-  } else {
-    constexpr int WAVES = TPR / 64;
-    v = group_sum<64>(v);
-    float* s = smem + turn * WAVES;
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0.f;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) v += s[w];
-    return v;
-  }
+  float none = 0.f;
+  row_sums<TPR>(v, none, smem, turn);
+  return v;
 }
 
 }  // namespace cpd

@@ -204,6 +204,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int parts,
                                                       u64* keys) {
   constexpr int VEC = Vec16<T>::N;
   constexpr int TPR = WAVES * 64;
+  constexpr int LOADS = 4;
   __shared__ Soft softs[WAVES];
   __shared__ u64 lists[TOP && WAVES > 1 ? WAVES : 1][kMostTop];
   const int tid = threadIdx.x % TPR;
@@ -235,13 +236,24 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int parts,
     const int to = a.vocab - from < per ? a.vocab : from + per;
     const T* x = static_cast<const T*>(a.x) + row * a.ld;
     Soft v = {-INFINITY, 0.f, 0.f};
-    for (int base = from; base < to; base += TPR * VEC) {
-      const int at = base + tid * VEC;
-      float u[VEC];
-      load_vec<T>(x + at, to - at, -INFINITY, u);
-      float big = u[0];
+    // four loads a thread at a time, one rescaling for all of them
+    for (int base = from; base < to; base += TPR * VEC * LOADS) {
+      float u[LOADS][VEC];
 #pragma unroll
-      for (int i = 1; i < VEC; ++i) big = fmaxf(big, u[i]);
+      for (int c = 0; c < LOADS; ++c) {
+        const int at = base + (c * TPR + tid) * VEC;
+        load_vec<T>(x + at, to - at, -INFINITY, u[c]);
+      }
+      float tops[LOADS];
+#pragma unroll
+      for (int c = 0; c < LOADS; ++c) {
+        tops[c] = u[c][0];
+#pragma unroll
+        for (int i = 1; i < VEC; ++i) tops[c] = fmaxf(tops[c], u[c][i]);
+      }
+      float big = tops[0];
+#pragma unroll
+      for (int c = 1; c < LOADS; ++c) big = fmaxf(big, tops[c]);
       if (big > v.m) {
         const float d = v.m == -INFINITY ? 0.f : near(v.m - big);
         const float f = v.m == -INFINITY ? 0.f : fast_exp(d);
@@ -251,21 +263,28 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int parts,
       }
       const float about = v.m == -INFINITY ? 0.f : v.m;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float d = u[i] - about;
-        const float e = fast_exp(d);
-        v.s += e;
-        v.a += e * near(d);
-      }
-      if (TOP) {
-        const float bar = top.bar();
-        bool some = false;
+      for (int c = 0; c < LOADS; ++c)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) some |= !(u[i] <= bar);
-        if (__ballot(some && at < to)) {
+        for (int i = 0; i < VEC; ++i) {
+          const float d = u[c][i] - about;
+          const float e = fast_exp(d);
+          v.s += e;
+          v.a += e * near(d);
+        }
+      if (TOP) {
+        // a NaN is passed over by the maximum, but it makes the sum one
+        const bool odd = v.s != v.s;
+#pragma unroll
+        for (int c = 0; c < LOADS; ++c) {
+          // Values equal to the bar came later than what set it, within a
+          // vector too, as long as the bar is the one from before the vector.
+          const float bar = top.bar();
+          if (!__ballot(odd || !(tops[c] <= bar))) continue;
+          const int at = base + (c * TPR + tid) * VEC;
 #pragma unroll
           for (int i = 0; i < VEC; ++i)
-            top.offer(at + i < to ? key_of(u[i], at + i) : 0);
+            if (__ballot(!(u[c][i] <= bar)))
+              top.offer(at + i < to ? key_of(u[c][i], at + i) : 0);
         }
       }
     }
@@ -301,10 +320,18 @@ __global__ __launch_bounds__(256) void logprob_join_kernel(
     v = {p.m, p.s, p.a};
   }
   v = wave_join(v);
-  if (TOP)
-    for (int p = wave; p < parts; p += 4)
-      top.offer(top.lane < a.top ? keys[(row * parts + p) * a.top + top.lane]
-                                 : 0);
+  if (TOP) {
+    u64 key[16];  // all of them in flight
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int p = wave + 4 * i;
+      key[i] = p < parts && top.lane < a.top
+                   ? keys[(row * parts + p) * a.top + top.lane]
+                   : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top.offer(key[i]);
+  }
   block_join<4, TOP>(v, top, softs, lists);
   if (wave == 0) finish<4, TOP>(a, row, target, v, top);
 }

@@ -40,7 +40,6 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_fwd_kernel(
   constexpr int ROWS = TPR <= 64 ? 256 / TPR : 1;  // rows of a block
   __shared__ float smem[4 * (TPR <= 64 ? 1 : TPR / 64)];
   const int lane = threadIdx.x % TPR;
-  int turn = 0;
   for (long row0 = (long)blockIdx.x * ROWS; row0 < a.rows;
        row0 += (long)gridDim.x * ROWS) {
     const long row = row0 + threadIdx.x / TPR;
@@ -71,7 +70,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_fwd_kernel(
     for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sum += v[c][i];
-    const float mean = row_sum<TPR>(sum, smem, turn) / (float)a.cols;
+    const float mean = row_sum<TPR>(sum, smem, 0) / (float)a.cols;
     float sq = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -82,8 +81,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_fwd_kernel(
         sq += at + i < a.cols ? d * d : 0.f;
       }
     }
-    const float var = row_sum<TPR>(sq, smem, turn + 1) / (float)a.cols;
-    turn ^= 2;
+    const float var = row_sum<TPR>(sq, smem, 1) / (float)a.cols;
     const float rstd = 1.0f / sqrtf(var + a.eps);
     if (a.stats && lane == 0) {
       a.stats[row * 2] = mean;
@@ -113,7 +111,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_fwd_kernel(
 template <typename T>
 __global__ __launch_bounds__(1024) void norm_fwd_loop_kernel(NormArgs a) {
   constexpr int VEC = Vec16<T>::N;
-  __shared__ float smem[2 * 16];
+  __shared__ float smem[4 * 16];
   // (the launcher starts one block for every row)
   const long row = blockIdx.x;
   const T* x = static_cast<const T*>(a.x) + row * a.x_ld;
@@ -176,8 +174,10 @@ __global__ __launch_bounds__(1024) void norm_fwd_loop_kernel(NormArgs a) {
 
 // Backward: each block walks rows gridDim.x apart and keeps its share of
 // dweight and dbias in registers (a thread has the same columns in every
-// row), so the data is read once for all three gradients.  The blocks' shares
-// go to `partial` and are added in a fixed order: no atomics.
+// row), so the data is read once for all three gradients; the next row is
+// ordered before this one is worked on, since the two sums over the row leave
+// memory idle otherwise.  The blocks' shares go to `partial` and are added in a
+// fixed order: no atomics.
 template <typename T, int TPR, int CH>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_bwd_kernel(
     NormGradArgs a) {
@@ -185,28 +185,32 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_bwd_kernel(
   constexpr int ROWS = TPR <= 64 ? 256 / TPR : 1;
   __shared__ float smem[4 * (TPR <= 64 ? 1 : TPR / 64)];
   const int lane = threadIdx.x % TPR;
-  float dw[CH][VEC] = {}, db[CH][VEC] = {};
-  int turn = 0;
-  for (long row0 = (long)blockIdx.x * ROWS; row0 < a.rows;
-       row0 += (long)gridDim.x * ROWS) {
-    const long row = row0 + threadIdx.x / TPR;
-    if (row >= a.rows) break;  // only where a row is within a wave (ROWS > 1)
-    const T* s = static_cast<const T*>(a.s) + row * a.s_ld;
-    const T* dy = static_cast<const T*>(a.dy) + row * a.dy_ld;
-    const float mean = a.stats[row * 2], rstd = a.stats[row * 2 + 1];
-    float h[CH][VEC], g[CH][VEC];
-    float sg = 0.f, sgh = 0.f;
+  const long stride = (long)gridDim.x * ROWS;
+  struct Row {
+    typename Vec16<T>::type s[CH], dy[CH], ds[CH];
+    float mean, rstd;
+  };
+  auto fetch = [&](long row, Row& r) {
+    if (row >= a.rows) return;
+    r.mean = a.stats[row * 2];
+    r.rstd = a.stats[row * 2 + 1];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int at = (c * TPR + lane) * VEC;
-      load_vec<T>(s + at, a.cols - at, mean, h[c]);
-      if (a.dy) {
-        load_vec<T>(dy + at, a.cols - at, 0.f, g[c]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) g[c][i] = 0.f;
-      }
+      const int at = (c * TPR + lane) * VEC, left = a.cols - at;
+      r.s[c] = load_raw<T>(static_cast<const T*>(a.s) + row * a.s_ld + at, left);
+      r.dy[c] = load_raw<T>(static_cast<const T*>(a.dy) + row * a.dy_ld + at,
+                            a.dy ? left : 0);
+      r.ds[c] = load_raw<T>(static_cast<const T*>(a.ds) + row * a.ds_ld + at,
+                            a.ds ? left : 0);
     }
+  };
+  float dw[CH][VEC] = {}, db[CH][VEC] = {};
+  int turn = 0;
+  auto work = [&](long row, const Row& r) {
+    // (ROWS > 1: a row's threads are within a wave, and leave together)
+    if (row >= a.rows) return;
+    float h[CH][VEC], g[CH][VEC];
+    float sg = 0.f, sgh = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int at = (c * TPR + lane) * VEC;
@@ -214,7 +218,8 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_bwd_kernel(
       if (a.weight) load_learned<VEC>(a.weight, a.wdt, at, a.cols - at, w);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        h[c][i] = (h[c][i] - mean) * rstd;
+        h[c][i] = ((float)r.s[c][i] - r.mean) * r.rstd;
+        g[c][i] = (float)r.dy[c][i];
         dw[c][i] += g[c][i] * h[c][i];
         db[c][i] += g[c][i];
         if (a.weight) g[c][i] *= w[i];
@@ -222,28 +227,32 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_bwd_kernel(
         sgh += g[c][i] * h[c][i];
       }
     }
-    // two sums, two barriers a row; the slots alternate between rows
-    sg = row_sum<TPR>(sg, smem, turn) / (float)a.cols;
-    sgh = row_sum<TPR>(sgh, smem, turn + 1) / (float)a.cols;
-    turn ^= 2;
+    row_sums<TPR>(sg, sgh, smem, turn);
+    turn ^= 1;
+    sg /= (float)a.cols;
+    sgh /= (float)a.cols;
     T* dx = static_cast<T*>(a.dx) + row * a.cols;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int at = (c * TPR + lane) * VEC;
       if (at >= a.cols) break;
       float o[VEC];
-      if (a.ds) {
-        const T* ds = static_cast<const T*>(a.ds) + row * a.ds_ld;
-        load_vec<T>(ds + at, a.cols - at, 0.f, o);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = 0.f;
-      }
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
-        o[i] += rstd * (g[c][i] - sg - h[c][i] * sgh);
+        o[i] = (float)r.ds[c][i] + r.rstd * (g[c][i] - sg - h[c][i] * sgh);
       store_vec<T>(dx + at, a.cols - at, o);
     }
+  };
+  Row r0, r1;
+  const long first = (long)blockIdx.x * ROWS;
+  const int mine = threadIdx.x / TPR;
+  fetch(first + mine, r0);
+  for (long row = first; row < a.rows; row += 2 * stride) {
+    fetch(row + stride + mine, r1);
+    work(row + mine, r0);
+    if (row + stride >= a.rows) break;
+    fetch(row + 2 * stride + mine, r0);
+    work(row + stride + mine, r1);
   }
   if (!a.partial) return;
   float* part = a.partial + (long)blockIdx.x * 2 * a.cols;
@@ -261,7 +270,6 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_bwd_kernel(
   } else {
     // the block's rows share columns: add them up through LDS, in order
     __shared__ float add[ROWS][TPR * VEC + 1];
-    const int mine = threadIdx.x / TPR;
 #pragma unroll
     for (int c = 0; c < 2 * CH; ++c) {
       const int base = (c >> 1) * TPR * VEC;
@@ -282,7 +290,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_bwd_kernel(
 template <typename T>
 __global__ __launch_bounds__(1024) void norm_bwd_loop_kernel(NormGradArgs a) {
   constexpr int VEC = Vec16<T>::N;
-  __shared__ float smem[2 * 16];
+  __shared__ float smem[4 * 16];
   const long row = blockIdx.x;
   const T* s = static_cast<const T*>(a.s) + row * a.s_ld;
   const T* dy = static_cast<const T*>(a.dy) + row * a.dy_ld;
@@ -342,25 +350,35 @@ __global__ __launch_bounds__(256) void norm_bwd_cols_kernel(NormGradArgs a) {
   part[a.cols + col] = db;
 }
 
-// Adds the blocks' shares: 64 columns a block, 16 strips of rows.
+// Adds the blocks' shares: 32 columns a block, 32 strips of rows, each thread
+// with four loads in flight.
 __global__ __launch_bounds__(1024) void norm_bwd_join_kernel(
     const float* __restrict__ partial, int blocks, int cols, void* dweight,
     void* dbias, Dt wdt) {
-  __shared__ float add[16][65];
-  const int j = threadIdx.x & 63, strip = threadIdx.x >> 6;
-  const long col = (long)blockIdx.x * 64 + j;  // over [2, cols] flattened
-  float t = 0.f;
-  if (col < 2L * cols)
-    for (int b = strip; b < blocks; b += 16)
-      t += partial[(long)b * 2 * cols + col];
-  add[strip][j] = t;
-  __syncthreads();
-  if (strip == 0 && col < 2L * cols) {
-    t = 0.f;
+  __shared__ float add[32][33];
+  const int j = threadIdx.x & 31, strip = threadIdx.x >> 5;
+  const long all = 2L * cols;
+  const long col = (long)blockIdx.x * 32 + j;  // over [2, cols] flattened
+  float t[4] = {};
+  if (col < all) {
+    const float* p = partial + col;
+    int b = strip;
+    for (; b + 96 < blocks; b += 128)
 #pragma unroll
-    for (int s = 0; s < 16; ++s) t += add[s][j];
-    void* to = col < cols ? dweight : dbias;
-    if (to) store_as(to, wdt, col < cols ? col : col - cols, t);
+      for (int q = 0; q < 4; ++q) t[q] += p[(b + q * 32) * all];
+    for (; b < blocks; b += 32) t[0] += p[b * all];
+  }
+  add[strip][j] = (t[0] + t[1]) + (t[2] + t[3]);
+  __syncthreads();
+  // a half wave a column now
+  const int mine = threadIdx.x >> 5;
+  float v = add[threadIdx.x & 31][mine];
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor(v, d, 32);
+  const long to = (long)blockIdx.x * 32 + mine;
+  if ((threadIdx.x & 31) == 0 && to < all) {
+    void* out = to < cols ? dweight : dbias;
+    if (out) store_as(out, wdt, to < cols ? to : to - cols, v);
   }
 }
 
@@ -442,7 +460,7 @@ void norm_backward(const NormGradArgs& a, hipStream_t st) {
   else
     backward_t<f16_t>(a, st);
   if (a.partial)
-    norm_bwd_join_kernel<<<dim3((2L * a.cols + 63) / 64), dim3(1024), 0, st>>>(
+    norm_bwd_join_kernel<<<dim3((2L * a.cols + 31) / 32), dim3(1024), 0, st>>>(
         a.partial, norm_grad_blocks(a.rows, a.cols, a.dt), a.cols, a.dweight,
         a.dbias, a.wdt);
 }
