@@ -107,16 +107,18 @@ __device__ __forceinline__ void store_as(void* p, Dt dt, long at, float v) {
     static_cast<f16_t*>(p)[at] = (f16_t)v;
 }
 
-// 16 bytes as they are; elements at or behind `left` are zero.
+// 16 bytes as they are; elements at or behind `left` are `fill`.
 template <typename T>
-__device__ __forceinline__ typename Vec16<T>::type load_raw(const T* p,
-                                                            int left) {
+__device__ __forceinline__ typename Vec16<T>::type load_raw(const T* p, int left,
+                                                            T fill = (T)0.f) {
   typedef typename Vec16<T>::type V;
   if (left >= Vec16<T>::N) return *reinterpret_cast<const V*>(p);
-  V v = {};
+  V v;
 #pragma unroll
-  for (int i = 0; i < Vec16<T>::N; ++i)
+  for (int i = 0; i < Vec16<T>::N; ++i) {
+    v[i] = fill;
     if (i < left) v[i] = p[i];
+  }
   return v;
 }
 

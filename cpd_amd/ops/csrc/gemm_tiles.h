@@ -57,7 +57,9 @@ __device__ __forceinline__ void copy_to_lds(const void* base, u32 off, u32 lds) 
 
 template <int N>
 __device__ __forceinline__ void wait_copies() {  // all but the newest N, and LDS reads
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+  // lgkmcnt(0) alone, in the form that the compiler takes note of
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ void block_barrier() {

@@ -371,21 +371,37 @@ __global__ __launch_bounds__(512, 2) void gemm_128_kernel(GemmArgs g, int tm,
     block_barrier();
     read(lds, f0);
   }
-  auto step = [&](int t, const Fragments& now, Fragments& next) {
-    if (t + 1 < to) {
-      if (t + 3 < to)
-        wait_copies<8>();
-      else
-        wait_copies<0>();
-      block_barrier();
-      if (t + 4 < to) copy(t + 4);
-      read(lds + ((t + 1 - from) & 3) * (2 * kHalf), next);
-    }
+  // (No branch around the reads, and nothing moved across them: where the
+  // compiler cannot tell how many LDS reads are in flight, the matrix
+  // instructions wait for all of them, and left to itself it reads behind them.)
+  auto step = [&](int t, const Fragments& now, Fragments& next, auto steady) {
+    constexpr bool STEADY = decltype(steady)::value;
+    if (STEADY || t + 3 < to)
+      wait_copies<8>();
+    else
+      wait_copies<0>();
+    block_barrier();
+    if (STEADY || t + 4 < to) copy(t + 4);
+    read(lds + ((t + 1 - from) & 3) * (2 * kHalf), next);
+    __builtin_amdgcn_sched_barrier(0);
     multiply(now);
   };
-  for (int t = from; t < to; t += 2) {
-    step(t, f0, f1);
-    if (t + 1 < to) step(t + 1, f1, f0);
+  const std::true_type steady;
+  const std::false_type ending;
+  int t = from;
+  for (; t + 5 < to; t += 2) {
+    step(t, f0, f1, steady);
+    step(t + 1, f1, f0, steady);
+  }
+  for (; t + 2 < to; t += 2) {
+    step(t, f0, f1, ending);
+    step(t + 1, f1, f0, ending);
+  }
+  if (t + 1 < to) {
+    step(t, f0, f1, ending);
+    multiply(f1);
+  } else if (t < to) {
+    multiply(f0);
   }
   __syncthreads();
   if (left) {

@@ -18,7 +18,7 @@
 // read as a sorted list, one entry a lane, and compares a whole vector of
 // new values with the k-th entry before it does anything else.  For values in
 // no order that test fails about k log(n / k) times in n values; values that
-// keep rising would insert every one of them, which is slower but as right.
+// keep rising pass one and all, which is slower but as right.
 //
 // A row of -inf alone has log probability -inf, entropy 0 and no gradient.
 // NaN or +inf in a row makes its log probabilities NaN; among the
@@ -88,6 +88,17 @@ __device__ __forceinline__ u64 lane_key(u64 v, int lane) {
   return ((u64)hi << 32) | lo;
 }
 
+__device__ __forceinline__ u64 key_across(u64 v, int d) {
+  const u32 lo = __shfl_xor((u32)v, d, 64), hi = __shfl_xor((u32)(v >> 32), d, 64);
+  return ((u64)hi << 32) | lo;
+}
+
+// The larger of two lanes' keys, or the smaller, to each its own.
+__device__ __forceinline__ u64 exchange(u64 key, int d, bool larger) {
+  const u64 other = key_across(key, d);
+  return (other > key) == larger ? other : key;
+}
+
 // The wave's list: lane i holds the i-th entry.
 struct Top {
   u64 mine, least;  // this lane's entry; the k-th entry
@@ -102,6 +113,16 @@ struct Top {
   __device__ __forceinline__ float bar() const {
     return least ? key_value(least) : NAN;
   }
+  // Joins a list in order, the largest first, one key a lane.
+  __device__ __forceinline__ void join_list(u64 key) {
+    // the larger of the i-th and the other's i-th from its end: the 64 best,
+    // rising and falling once, which six exchanges put in order
+    const u64 back = key_across(key, 63);
+    mine = back > mine ? back : mine;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) mine = exchange(mine, d, !(lane & d));
+    least = lane_key(mine, k - 1);
+  }
   __device__ __forceinline__ void insert(u64 key) {
     const int at = __popcll(__ballot(mine > key));
     // the entry of the lane below (wave_shr:1)
@@ -113,13 +134,26 @@ struct Top {
     mine = lane < at ? mine : lane == at ? key : below;
     least = lane_key(mine, k - 1);
   }
-  // every lane's key, best ones kept
+  // Every lane's key, the best ones kept: a few are inserted one by one, many
+  // are put in order together (21 exchanges) and joined.  (For a list of one or
+  // two few of the many would be inserted.)
   __device__ __forceinline__ void offer(u64 key) {
-    u64 mask;
-    while ((mask = __ballot(key > least)) != 0) {
+    u64 mask = __ballot(key > least);
+    if (__popcll(mask) > 24 && k > 2) {
+      key = key > least ? key : 0;
+#pragma unroll 1
+      for (int size = 2; size <= 64; size *= 2)
+#pragma unroll 1
+        for (int d = size / 2; d > 0; d >>= 1)
+          key = exchange(key, d, !(lane & d) == !(lane & size));
+      join_list(key);
+      return;
+    }
+    while (mask) {
       const int from = __ffsll(mask) - 1;
       insert(lane_key(key, from));
       if (lane == from) key = 0;
+      mask = __ballot(key > least);
     }
   }
 };
@@ -193,9 +227,72 @@ __device__ __forceinline__ void block_join(Soft& v, Top& top, Soft* softs,
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) {
       v = join(v, softs[w]);
-      if (TOP) top.offer(top.lane < top.k ? lists[w][top.lane] : 0);
+      if (TOP) top.join_list(lists[w][top.lane]);
     }
   }
+}
+
+struct Found {
+  float value[64][4];  // 16 bytes of T
+  int at[64], done[64];
+};
+
+// Offers a wave's vectors, one a lane, the first of them from index `from` on.
+// (Rare, so it is kept small: it works through LDS and in loops, and hides its
+// lane number from the compiler, which otherwise works out everything that
+// depends on it ahead of the row and holds it in 80 registers.)
+template <typename T>
+__device__ __forceinline__ void search(Top& top,
+                                       const typename Vec16<T>::type* seen,
+                                       Found& found, bool odd, int from, int to) {
+  constexpr int VEC = Vec16<T>::N;
+  asm volatile("" : "+v"(top.lane));
+  const typename Vec16<T>::type u = seen[top.lane];
+  const int at = from + top.lane * VEC;
+  // the largest value, where it is first, and the next one
+  float most = -INFINITY, second = -INFINITY;
+  int done = -1;
+#pragma unroll
+  for (int i = VEC - 1; i >= 0; --i) {
+    const float y = (float)u[i];
+    if (y >= most) {
+      second = done >= 0 ? most : second;
+      most = y;
+      done = i;
+    } else {
+      second = fmaxf(second, y);
+    }
+  }
+  bool mine = odd || !(most <= top.bar());
+  u64 mask = __ballot(mine);
+  if (!mask) return;
+  if (__popcll(mask) > 8 && !__ballot(odd)) {
+    // Many pass, as at a row's start: their largest values first, after which
+    // most of the others do not.  (One that equals the bar may come before
+    // what set it here.)
+    top.offer(mine && at + done < to ? key_of(most, at + done) : 0);
+    mine = mine && !(second < top.bar());
+    mask = __ballot(mine);
+    if (!mask) return;
+  } else {
+    done = -1;
+  }
+  // the vectors that are left side by side, and from there one value a lane
+  const int rank = __popcll(mask & ((1ull << top.lane) - 1));
+  if (mine) {
+    *reinterpret_cast<typename Vec16<T>::type*>(found.value[rank]) = u;
+    found.at[rank] = at;
+    found.done[rank] = done;
+  }
+  __builtin_amdgcn_wave_barrier();
+  const int many = __popcll(mask) * VEC;
+  for (int i = top.lane; i - top.lane < many; i += 64) {
+    const int slot = i / VEC & 63, index = found.at[slot] + i % VEC;
+    const bool in = i < many && index < to && found.done[slot] != i % VEC;
+    const float value = (float)reinterpret_cast<const T*>(found.value)[i & (64 * VEC - 1)];
+    top.offer(in ? key_of(value, index) : 0);
+  }
+  __builtin_amdgcn_wave_barrier();
 }
 
 template <typename T, int WAVES, bool TOP>
@@ -204,15 +301,21 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int parts,
                                                       u64* keys) {
   constexpr int VEC = Vec16<T>::N;
   constexpr int TPR = WAVES * 64;
-  constexpr int LOADS = 4;
+  // (with alternatives 16-bit rows have registers for two: with four and 138
+  // registers 16384 rows of 8192 with five of them took 225 us instead of 196)
+  constexpr int LOADS = TOP && sizeof(T) == 2 ? 2 : 4;
   __shared__ Soft softs[WAVES];
   __shared__ u64 lists[TOP && WAVES > 1 ? WAVES : 1][kMostTop];
+  __shared__ typename Vec16<T>::type seen[TOP ? 4 : 1][LOADS][64];
+  __shared__ Found found[TOP ? 4 : 1];
+  // (in a scalar register: what a row or a wave shares stays out of the others)
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tid = threadIdx.x % TPR;
   const long jobs = a.rows * parts;
   Top top;
   for (long job0 = (long)blockIdx.x * (256 / TPR); job0 < jobs;
        job0 += (long)gridDim.x * (256 / TPR)) {
-    const long job = job0 + threadIdx.x / TPR;
+    const long job = job0 + (WAVES == 1 ? wave : 0);
     if (job >= jobs) break;  // WAVES == 1 only: a whole wave leaves
     const long row = job / parts;
     const int64_t target = a.targets[row];
@@ -236,24 +339,25 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int parts,
     const int to = a.vocab - from < per ? a.vocab : from + per;
     const T* x = static_cast<const T*>(a.x) + row * a.ld;
     Soft v = {-INFINITY, 0.f, 0.f};
-    // four loads a thread at a time, one rescaling for all of them
+    // a few loads a thread at a time, one rescaling for all of them
     for (int base = from; base < to; base += TPR * VEC * LOADS) {
-      float u[LOADS][VEC];
+      typename Vec16<T>::type u[LOADS];
+      if (base + TPR * VEC * LOADS <= to) {
 #pragma unroll
-      for (int c = 0; c < LOADS; ++c) {
-        const int at = base + (c * TPR + tid) * VEC;
-        load_vec<T>(x + at, to - at, -INFINITY, u[c]);
+        for (int c = 0; c < LOADS; ++c)
+          u[c] = load_raw<T>(x + base + (c * TPR + tid) * VEC, VEC);
+      } else {
+#pragma unroll
+        for (int c = 0; c < LOADS; ++c) {
+          const int at = base + (c * TPR + tid) * VEC;
+          u[c] = load_raw<T>(x + at, to - at, (T)-INFINITY);
+        }
       }
-      float tops[LOADS];
+      float big = (float)u[0][0];
 #pragma unroll
-      for (int c = 0; c < LOADS; ++c) {
-        tops[c] = u[c][0];
+      for (int c = 0; c < LOADS; ++c)
 #pragma unroll
-        for (int i = 1; i < VEC; ++i) tops[c] = fmaxf(tops[c], u[c][i]);
-      }
-      float big = tops[0];
-#pragma unroll
-      for (int c = 1; c < LOADS; ++c) big = fmaxf(big, tops[c]);
+        for (int i = 0; i < VEC; ++i) big = fmaxf(big, (float)u[c][i]);
       if (big > v.m) {
         const float d = v.m == -INFINITY ? 0.f : near(v.m - big);
         const float f = v.m == -INFINITY ? 0.f : fast_exp(d);
@@ -266,7 +370,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int parts,
       for (int c = 0; c < LOADS; ++c)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          const float d = u[c][i] - about;
+          const float d = (float)u[c][i] - about;
           const float e = fast_exp(d);
           v.s += e;
           v.a += e * near(d);
@@ -274,17 +378,14 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int parts,
       if (TOP) {
         // a NaN is passed over by the maximum, but it makes the sum one
         const bool odd = v.s != v.s;
+        // Values equal to the bar come after what set it and do not pass.
+        if (__ballot(odd || !(big <= top.bar()))) {
 #pragma unroll
-        for (int c = 0; c < LOADS; ++c) {
-          // Values equal to the bar came later than what set it, within a
-          // vector too, as long as the bar is the one from before the vector.
-          const float bar = top.bar();
-          if (!__ballot(odd || !(tops[c] <= bar))) continue;
-          const int at = base + (c * TPR + tid) * VEC;
-#pragma unroll
-          for (int i = 0; i < VEC; ++i)
-            if (__ballot(!(u[c][i] <= bar)))
-              top.offer(at + i < to ? key_of(u[c][i], at + i) : 0);
+          for (int c = 0; c < LOADS; ++c) seen[wave][c][top.lane] = u[c];
+#pragma unroll 1
+          for (int c = 0; c < LOADS; ++c)
+            search<T>(top, seen[wave][c], found[wave], odd,
+                      base + (c * TPR + tid - top.lane) * VEC, to);
         }
       }
     }
@@ -330,7 +431,8 @@ __global__ __launch_bounds__(256) void logprob_join_kernel(
                    : 0;
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top.offer(key[i]);
+    for (int i = 0; i < 16; ++i)
+      if (wave + 4 * i < parts) top.join_list(key[i]);
   }
   block_join<4, TOP>(v, top, softs, lists);
   if (wave == 0) finish<4, TOP>(a, row, target, v, top);
