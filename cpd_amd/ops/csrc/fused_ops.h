@@ -103,6 +103,7 @@ struct GemmArgs {
 };
 // `along`: both operands are
 long gemm_work_floats(long m, long n, long k, Dt dt, bool along);
+constexpr long kMostFeatures = 1L << 22;
 // Whether a 16-bit product takes the operand as it lies (`rows` by k), 16
 // bytes at a time; if not, pad_rows makes a copy that it takes.  Floats are
 // taken as they lie, and so is everything along with gemm_few_rows.

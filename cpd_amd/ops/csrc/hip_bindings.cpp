@@ -309,21 +309,21 @@ Tensor logprob_bwd(const Tensor& x, const Tensor& targets, const Tensor& stats,
 // linear
 // ---------------------------------------------------------------------------
 
-constexpr int64_t kMostSize = (1L << 31) - 1024;
-
 cpd::Act act_of(int64_t act) {
   TORCH_CHECK_VALUE(act >= 0 && act <= 3, "unknown activation");
   return static_cast<cpd::Act>(act);
 }
 
+// m rows of k features in, n out: what the kernels count in 32 bits, for the
+// product and for both of its gradients.
 void check_sizes(int64_t m, int64_t n, int64_t k) {
-  TORCH_CHECK_VALUE(m < kMostSize && n < kMostSize && k < kMostSize,
-                    "linear takes sizes below 2^31 - 1024");
-  const int64_t tiles = ((m + 63) / 64) * ((n + 63) / 64);
-  TORCH_CHECK_VALUE(tiles < (1L << 24), "linear's output is too large");
-  // (a tile's 256 rows are reached with 32-bit offsets)
-  TORCH_CHECK_VALUE(n < (1L << 22) && k < (1L << 22),
+  TORCH_CHECK_VALUE(m < (1L << 31) - 8192, "linear takes less than 2^31 - 8192 rows");
+  TORCH_CHECK_VALUE(n < cpd::kMostFeatures && k < cpd::kMostFeatures,
                     "linear takes less than 2^22 features");
+  auto tiles = [](int64_t a, int64_t b) { return ((a + 127) / 128) * ((b + 127) / 128); };
+  TORCH_CHECK_VALUE(tiles(m, n) < (1L << 22) && tiles(m, k) < (1L << 22) &&
+                        tiles(n, k) < (1L << 22),
+                    "linear's tensors are too large");
 }
 
 // The products of a call: operands as the kernels read them, and workspaces,
@@ -424,8 +424,6 @@ std::vector<Tensor> linear_bwd(const Tensor& dy, const Tensor& x,
                     "the output's gradient has shape ", dy.sizes());
   const int64_t m = r.rows;
   check_sizes(m, n, k);
-  check_sizes(m, k, n);
-  check_sizes(n, k, m);
   Rows g = rows_of(dy);
   g.rows = m;
   Tensor dx, dw, db, dz, partial;
@@ -450,15 +448,19 @@ std::vector<Tensor> linear_bwd(const Tensor& dy, const Tensor& x,
     zr = rows_of(*z);
     p.z = zr.p;
     p.z_ld = zr.ld;
-    if (need_x || need_w) {
-      // rows a multiple of 16 bytes apart, as the products read them
-      g.ld = (n + 7) / 8 * 8;
-      dz = at::empty({m, g.ld}, x.options());
-      p.dz = dz.mutable_data_ptr();
-      p.dz_ld = g.ld;
-      g.p = p.dz;
-      g.keep = dz;
-    }
+  }
+  // dz, or a copy of a dy that the products do not take as it lies: rows a
+  // multiple of 16 bytes apart
+  const bool fits =
+      dt == Dt::f32 || ((!need_x || cpd::gemm_takes({g.p, g.ld, false, false}, m)) &&
+                        (!need_w || cpd::gemm_takes({g.p, g.ld, true, false}, n)));
+  if ((need_x || need_w) && (p.act != cpd::Act::none || !fits)) {
+    g.ld = (n + 7) / 8 * 8;
+    dz = at::empty({m, g.ld}, x.options());
+    p.dz = dz.mutable_data_ptr();
+    p.dz_ld = g.ld;
+    g.p = p.dz;
+    g.keep = dz;
   }
   if (need_b) {
     p.dbias = db.mutable_data_ptr();

@@ -826,11 +826,15 @@ __global__ __launch_bounds__(256) void act_grad_kernel(ActGradArgs a,
   __syncthreads();
   if (wave == 0) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i)
-      if (i < left)
-        a.partial[(long)blockIdx.y * a.n + col + i] =
-            add[0][i * 64 + lane] + add[1][i * 64 + lane] +
-            add[2][i * 64 + lane] + add[3][i * 64 + lane];
+    for (int i = 0; i < VEC; ++i) {
+      const float t = add[0][i * 64 + lane] + add[1][i * 64 + lane] +
+                      add[2][i * 64 + lane] + add[3][i * 64 + lane];
+      if (i >= left) continue;
+      if (gridDim.y == 1)
+        store_as(a.dbias, a.bias_dt, col + i, t);
+      else
+        a.partial[(long)blockIdx.y * a.n + col + i] = t;
+    }
   }
 }
 
@@ -867,7 +871,8 @@ long gemm_work_floats(long m, long n, long k, Dt dt, bool along) {
 }
 
 bool gemm_takes(const Operand& o, long rows) {
-  return (uintptr_t)o.p % 16 == 0 && o.ld % 8 == 0 &&
+  // (a tile's 256 rows are reached with 32-bit offsets)
+  return (uintptr_t)o.p % 16 == 0 && o.ld % 8 == 0 && o.ld < kMostFeatures &&
          (!o.across || rows % 8 == 0 || o.padded);
 }
 
@@ -904,6 +909,7 @@ void pad_rows(const void* from, long ld, void* to, long to_ld, int rows,
 }
 
 int act_grad_slices(int m, int n, Dt dt) {
+  if (m <= 64) return 1;  // sixteen rows a wave: no second launch to join slices
   const int width = 64 * 16 / dt_size(dt);
   const int across = (n + width - 1) / width;
   int slices = (2048 + across - 1) / across;  // eight blocks a CU
@@ -923,7 +929,7 @@ void act_grad(const ActGradArgs& a, hipStream_t st) {
     act_grad_kernel<bf16_t><<<grid, dim3(256), 0, st>>>(a, per);
   else
     act_grad_kernel<f16_t><<<grid, dim3(256), 0, st>>>(a, per);
-  if (a.dbias)
+  if (a.dbias && slices > 1)
     column_join_kernel<<<dim3((a.n + 63) / 64), dim3(256), 0, st>>>(
         a.partial, slices, a.n, a.dbias, a.bias_dt);
 }

@@ -33,7 +33,7 @@ from cpd_amd.parallel import DistModule, dist_init
 from cpd_amd.trainers.core import LPTrainStep
 from cpd_amd.utils import (AverageMeter, DistributedGivenIterationSampler,
                            DistributedSampler, LARS, accuracy, load_state,
-                           save_checkpoint)
+                           save_checkpoint, token_logprobs)
 from cpd_amd.utils.scalars import ScalarLogger
 
 
@@ -49,6 +49,10 @@ def parse_args(argv=None):
     p.add_argument('--use_APS', action='store_true')
     p.add_argument('--use_kahan', action='store_true')
     p.add_argument('-e', '--evaluate', action='store_true')
+    p.add_argument('--val_stats', action='store_true',
+                   help='validation from one read of the logits '
+                        '(token_logprobs): loss, top-1, top-5 and the mean '
+                        'entropy of the predictions')
     p.add_argument('--emulate_node', default=1, type=int)
     p.add_argument('--mode', choices=['ring', 'sequential'], default='ring')
     p.add_argument('--overlap', type=int, default=0,
@@ -172,7 +176,8 @@ def main(argv=None):
                             pin_memory=True, sampler=val_sampler)
 
     if args.evaluate:
-        validate(val_loader, model, criterion, device, world_size, rank)
+        validate(val_loader, model, criterion, device, world_size, rank,
+                 args.val_stats)
         return
 
     train(args, train_loader, val_loader, dm, model, criterion, optimizer,
@@ -224,7 +229,7 @@ def train(args, train_loader, val_loader, dm, model, criterion, optimizer,
                 scalars.add_scalar('lr', lr, curr_step)
             if curr_step % args.val_freq == 0:
                 prec1 = validate(val_loader, model, criterion, device,
-                                 world_size, rank)
+                                 world_size, rank, args.val_stats)
                 model.train()
                 if rank == 0:
                     scalars.add_scalar('acc1', prec1, curr_step)
@@ -241,28 +246,39 @@ def train(args, train_loader, val_loader, dm, model, criterion, optimizer,
                     }, is_best, args.save_path)
 
 
-def validate(val_loader, model, criterion, device, world_size, rank):
+def validate(val_loader, model, criterion, device, world_size, rank,
+             val_stats=False):
     import torch.distributed as dist
 
     model.eval()
     losses, top1, top5 = AverageMeter(0), AverageMeter(0), AverageMeter(0)
+    entropies = AverageMeter(0)
     with torch.no_grad():
         for x, y in val_loader:
             x = x.to(device, non_blocking=True)
             y = y.to(device, non_blocking=True)
             out = model(x)
-            loss = criterion(out, y)
-            prec1, prec5 = accuracy(out, y, topk=(1, 5))
+            if val_stats:
+                said = token_logprobs(out, y, top_k=5)
+                loss = -said.logprobs.mean()
+                hits = (said.top_ids == y[:, None]).float() * 100.0
+                prec1, prec5 = hits[:, 0].mean(), hits.sum(1).mean()
+                entropies.update(float(said.entropy.mean()))
+            else:
+                loss = criterion(out, y)
+                prec1, prec5 = accuracy(out, y, topk=(1, 5))
             losses.update(float(loss))
             top1.update(float(prec1))
             top5.update(float(prec5))
-    stats = torch.tensor([losses.avg, top1.avg, top5.avg], device=device)
+    stats = torch.tensor([losses.avg, top1.avg, top5.avg, entropies.avg],
+                         device=device)
     if dist.is_available() and dist.is_initialized():
         dist.all_reduce(stats)
         stats /= world_size
     if rank == 0:
         print(f'* All Loss {stats[0]:.4f} Prec@1 {stats[1]:.3f} '
-              f'Prec@5 {stats[2]:.3f}', flush=True)
+              f'Prec@5 {stats[2]:.3f}'
+              + (f' Entropy {stats[3]:.4f}' if val_stats else ''), flush=True)
     return float(stats[1])
 
 

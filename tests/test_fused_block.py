@@ -398,6 +398,57 @@ def test_linear(device, dtype, m, k, n):
     run_linear(device, dtype, m, k, n)
 
 
+# sizes that the largest tiles are taken for, forward, in dx and in dW; k of
+# less than a tile, one, two and three tiles, and some more
+@pytest.mark.gpu
+@on_types
+@pytest.mark.parametrize("m,k,n", [
+    (4100, 40, 4100), (4100, 64, 4100), (4100, 128, 4100), (4100, 192, 4100),
+    (4100, 330, 4099), (4096, 4100, 330), (330, 4100, 4096),
+    (2050, 1000, 700)])
+def test_linear_large(dtype, m, k, n):
+    """Whole numbers, so that every sum is exact: equal to the formula in 64
+    bits, rounded once."""
+    g = torch.Generator(device="cuda").manual_seed(m + k + n)
+    draw = lambda *s: torch.randint(  # noqa: E731
+        -2, 3, s, generator=g, device="cuda").to(dtype)
+    x, w, b, res, dy = draw(m, k), draw(n, k), draw(n) + 0.5, draw(m, n), \
+        draw(m, n)
+    for v in (x, w, b, res):
+        v.requires_grad_(True)
+    y = fused_linear(x, w, b, "relu", res)
+    got = torch.autograd.grad(y, [x, w, b], dy)
+    x64, w64, dy64 = (v.detach().double() for v in (x, w, dy))
+    z = x64 @ w64.t() + b.detach().double()
+    assert torch.equal(y, (z.clamp_min(0) + res.detach().double()).to(dtype))
+    dz = torch.where(z > 0, dy64, 0.0)
+    for a, c in zip(got, (dz @ w64, dz.t() @ x64, dz.sum(0))):
+        assert torch.equal(a, c.to(dtype))
+
+
+@pytest.mark.gpu
+def test_linear_rows_far_apart():
+    """Rows 2^23 elements apart, more than a tile's offsets reach."""
+    wide = torch.zeros(140, 1 << 23, dtype=torch.bfloat16, device="cuda")
+    x = wide[:, :128]
+    x.copy_(torch.randint(-2, 3, (140, 128), device="cuda"))
+    w = torch.randint(-2, 3, (200, 128), device="cuda").bfloat16()
+    y = fused_linear(x, w)
+    assert torch.equal(y, (x.double() @ w.double().t()).bfloat16())
+    dx, dw = (v.detach().requires_grad_(True) for v in (x, w))
+    fused_linear(dx, dw).backward(torch.ones_like(y))
+    assert torch.equal(dw.grad, x.double().sum(0).bfloat16().expand(200, 128))
+
+
+@pytest.mark.parametrize("m,k,n", [(4, 1 << 22, 2), (4, 2, 1 << 22)])
+@pytest.mark.gpu
+def test_linear_refuses_sizes(m, k, n):
+    x = torch.zeros(m, k, dtype=torch.float16, device="cuda")
+    w = torch.zeros(n, k, dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError):
+        fused_linear(x, w)
+
+
 @on_devices
 @on_types
 @pytest.mark.parametrize("act", ACTS)
@@ -838,6 +889,34 @@ def test_logprobs_are_loss_and_accuracy(device):
     hits = got.top_ids == y[:, None]
     for k, acc in zip((1, 5), accuracy(out, y, topk=(1, 5))):
         assert abs(hits[:, :k].sum() * 100.0 / 64 - acc) < 1e-3
+
+
+@on_devices
+def test_trainer_validates_from_one_read(device, capsys):
+    """train_resnet18 --val_stats: the same line as without, and the
+    entropy."""
+    from cpd_amd.trainers.train_resnet18 import parse_args, validate
+    assert parse_args(["--val_stats"]).val_stats
+    assert not parse_args([]).val_stats
+    torch.manual_seed(6)
+    model = torch.nn.Linear(12, 10).to(device)
+    data = [(torch.randn(32, 12), torch.randint(0, 10, (32,)))
+            for _ in range(3)]
+    said = []
+    for stats in (False, True):
+        prec = validate(data, model, torch.nn.CrossEntropyLoss(),
+                        torch.device(device), 1, 0, stats)
+        said.append((prec, capsys.readouterr().out.split()))
+    (p, a), (q, b) = said
+    assert abs(p - q) < 1e-4
+    assert a[:3] == b[:3] == ["*", "All", "Loss"] and len(a) == 8
+    for i in (3, 5, 7):
+        assert abs(float(a[i]) - float(b[i])) < 2e-3
+    with torch.no_grad():
+        lp = torch.stack([torch.log_softmax(model(x.to(device)), -1)
+                          for x, _ in data])
+    assert b[8] == "Entropy"
+    assert abs(float(b[9]) + (lp.exp() * lp).sum(-1).mean().item()) < 1e-3
 
 
 # ---------------------------------------------------------------------------
