@@ -511,8 +511,14 @@ std::vector<Tensor> linear_bwd(const Tensor& dy, const Tensor& x,
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// Whether a node has to stand for this call: for a gradient, or for a tangent
+// of forward mode, which the node refuses and a bare call would lose.
+bool wants_grad(const Tensor& t) {
+  return (t.requires_grad() && at::GradMode::is_enabled()) ||
+         t._fw_grad(0).defined();
+}
 bool wants_grad(const OptTensor& t) {
-  return t.has_value() && t->defined() && t->requires_grad();
+  return t.has_value() && t->defined() && wants_grad(*t);
 }
 
 bool present(const OptTensor& t) { return t.has_value() && t->defined(); }
@@ -568,8 +574,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 std::vector<Tensor> layer_norm(const Tensor& x, const OptTensor& weight,
                                const OptTensor& bias, double eps,
                                const OptTensor& residual) {
-  if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) ||
-                                     wants_grad(bias) || wants_grad(residual)))
+  if (wants_grad(x) || wants_grad(weight) || wants_grad(bias) || wants_grad(residual))
     return LayerNorm::apply(x, weight, bias, eps, residual);
   auto out = norm_fwd(x, weight, bias, eps, residual);
   out.resize(residual ? 2 : 1);
@@ -610,9 +615,7 @@ struct Linear : torch::autograd::Function<Linear> {
 
 Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias,
               int64_t act, const OptTensor& residual) {
-  if (at::GradMode::is_enabled() &&
-      (x.requires_grad() || weight.requires_grad() || wants_grad(bias) ||
-       wants_grad(residual)))
+  if (wants_grad(x) || wants_grad(weight) || wants_grad(bias) || wants_grad(residual))
     return Linear::apply(x, weight, bias, act, residual);
   return linear_fwd(x, weight, bias, act, residual, false)[0];
 }
@@ -641,7 +644,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
 // logprobs, entropy, and with top > 0 ids and log probabilities
 std::vector<Tensor> token_logprobs(const Tensor& x, const Tensor& targets,
                                    int64_t top, int64_t ignore) {
-  if (at::GradMode::is_enabled() && x.requires_grad())
+  if (wants_grad(x))
     return TokenLogprobs::apply(x, targets, top, ignore);
   auto out = logprob_fwd(x, targets, top, ignore);
   if (!top) return {out[0], out[1]};

@@ -835,19 +835,30 @@ __global__ __launch_bounds__(256) void act_grad_kernel(ActGradArgs a,
   }
 }
 
-__global__ __launch_bounds__(256) void column_join_kernel(
+// 32 columns a block, 32 strips of slices, each thread with four loads in
+// flight.
+__global__ __launch_bounds__(1024) void column_join_kernel(
     const float* __restrict__ partial, int slices, int n, void* out, Dt dt) {
-  __shared__ float add[4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col = (int)(blockIdx.x * 64 + lane);
-  float t = 0.f;
-  if (col < n)
-    for (int s = wave; s < slices; s += 4) t += partial[(long)s * n + col];
-  add[wave][lane] = t;
+  __shared__ float add[32][33];
+  const int j = threadIdx.x & 31, strip = threadIdx.x >> 5;
+  const int col = (int)blockIdx.x * 32 + j;
+  float t[4] = {};
+  if (col < n) {
+    const float* p = partial + col;
+    int s = strip;
+    for (; s + 96 < slices; s += 128)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) t[q] += p[(long)(s + q * 32) * n];
+    for (; s < slices; s += 32) t[0] += p[(long)s * n];
+  }
+  add[strip][j] = (t[0] + t[1]) + (t[2] + t[3]);
   __syncthreads();
-  if (wave == 0 && col < n)
-    store_as(out, dt, col,
-             add[0][lane] + add[1][lane] + add[2][lane] + add[3][lane]);
+  // a half wave a column now
+  float v = add[j][strip];
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor(v, d, 32);
+  const int to = (int)blockIdx.x * 32 + strip;
+  if (j == 0 && to < n) store_as(out, dt, to, v);
 }
 
 }  // namespace
@@ -927,7 +938,7 @@ void act_grad(const ActGradArgs& a, hipStream_t st) {
   else
     act_grad_kernel<f16_t><<<grid, dim3(256), 0, st>>>(a, per);
   if (a.dbias && slices > 1)
-    column_join_kernel<<<dim3((a.n + 63) / 64), dim3(256), 0, st>>>(
+    column_join_kernel<<<dim3((a.n + 31) / 32), dim3(1024), 0, st>>>(
         a.partial, slices, a.n, a.dbias, a.bias_dt);
 }
 

@@ -21,9 +21,9 @@
 // keep rising pass one and all, which is slower but as right.
 //
 // Without alternatives 4096 rows of 50021 bf16 take 95 us (4.3 TB/s) forward and
-// 150 backward (5.4 TB/s).  Alternatives add the work of inserting them: 2048
-// rows of 131072 fp16 take 104 us, 124 with one, 153 with five, 194 with
-// sixteen, 300 with 64.
+// 149 backward (5.5 TB/s).  Alternatives add the work of inserting them: 2048
+// rows of 131072 fp16 take 104 us, 123 with one, 154 with five, 195 with
+// sixteen, 305 with 64.
 //
 // A row of -inf alone has log probability -inf, entropy 0 and no gradient.
 // NaN or +inf in a row makes its log probabilities NaN; among the
@@ -443,15 +443,24 @@ __global__ __launch_bounds__(256) void logprob_join_kernel(
   if (wave == 0) finish<4, TOP>(a, row, target, v, top);
 }
 
-template <typename T>
+// WAVES = 1: a wave has a whole row; 4: a block has one of its `chunks`.  32768
+// rows of 1000 take 38 us in 16 bits and 41 in 32 with a wave a row, 96 and 54
+// with a block; longer rows than a wave takes at once have a block's bandwidth.
+template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void logprob_bwd_kernel(LogprobGradArgs a,
                                                           int chunks) {
   constexpr int VEC = Vec16<T>::N;
+  constexpr int TPR = WAVES * 64;
   constexpr int UNROLL = 4;
+  const int tid = threadIdx.x % TPR;
   const long jobs = a.rows * chunks;
-  for (long job = blockIdx.x; job < jobs; job += gridDim.x) {
-    const long row = job / chunks;
-    const int base = (int)(job - row * chunks) * (256 * VEC * UNROLL);
+  // (in a scalar register, as everything that a row shares then is)
+  const int mine =
+      WAVES == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  for (long job = (long)blockIdx.x * (256 / TPR) + mine; job < jobs;
+       job += (long)gridDim.x * (256 / TPR)) {
+    const long row = WAVES == 1 ? job : job / chunks;
+    const int base = (int)(job - row * chunks) * (TPR * VEC * UNROLL);
     const int64_t target = a.targets[row];
     const T* x = static_cast<const T*>(a.x) + row * a.ld;
     T* dx = static_cast<T*>(a.dx) + row * a.vocab;
@@ -461,29 +470,37 @@ __global__ __launch_bounds__(256) void logprob_bwd_kernel(LogprobGradArgs a,
     const float gent = a.gentropy ? a.gentropy[row] : 0.f;
     if (target < 0 || target >= a.vocab) glp = NAN;
     const float c0 = -(glp + gent * (a.gentropy ? a.entropy[row] : 0.f));
-    float u[UNROLL][VEC];
+    // (all of a job's loads in flight at once: none under a condition but at a
+    // row's end, and none across them)
+    const bool whole = base + TPR * VEC * UNROLL <= a.vocab;
+    typename Vec16<T>::type u[UNROLL] = {};
     if (!skip) {
+      if (whole) {
 #pragma unroll
-      for (int c = 0; c < UNROLL; ++c) {
-        const int at = base + (c * 256 + (int)threadIdx.x) * VEC;
-        load_vec<T>(x + at, a.vocab - at, 0.f, u[c]);
+        for (int c = 0; c < UNROLL; ++c)
+          u[c] = load_raw<T>(x + base + (c * TPR + tid) * VEC, VEC);
+      } else {
+#pragma unroll
+        for (int c = 0; c < UNROLL; ++c) {
+          const int at = base + (c * TPR + tid) * VEC;
+          u[c] = load_raw<T>(x + at, a.vocab - at);
+        }
       }
     }
 #pragma unroll
     for (int c = 0; c < UNROLL; ++c) {
-      const int at = base + (c * 256 + (int)threadIdx.x) * VEC;
+      const int at = base + (c * TPR + tid) * VEC;
+      float d[VEC] = {};
+      if (!skip) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        float d = 0.f;
-        if (!skip) {
-          const float logp = (u[c][i] - m) - logs;
+        for (int i = 0; i < VEC; ++i) {
+          const float logp = ((float)u[c][i] - m) - logs;
           const float p = fast_exp(logp);
-          d = p == 0.f ? 0.f : p * (c0 - gent * logp);
-          if (at + i == target) d += glp;
+          d[i] = p == 0.f ? 0.f : p * (c0 - gent * logp);
+          if (at + i == target) d[i] += glp;
         }
-        u[c][i] = d;
       }
-      if (at < a.vocab) store_vec<T>(dx + at, a.vocab - at, u[c]);
+      if (at < a.vocab) store_vec<T>(dx + at, whole ? VEC : a.vocab - at, d);
     }
   }
 }
@@ -519,9 +536,13 @@ template <typename T>
 void backward_t(const LogprobGradArgs& a, hipStream_t st) {
   const int per = 256 * Vec16<T>::N * 4;
   const int chunks = (int)(((long)a.vocab + per - 1) / per);
-  const long jobs = a.rows * chunks;
-  const dim3 grid((unsigned)(jobs < (1 << 20) ? jobs : 1 << 20));
-  logprob_bwd_kernel<T><<<grid, dim3(256), 0, st>>>(a, chunks);
+  const bool wave = a.vocab <= per / 4;
+  const long blocks = wave ? (a.rows + 3) / 4 : a.rows * chunks;
+  const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20));
+  if (wave)
+    logprob_bwd_kernel<T, 1><<<grid, dim3(256), 0, st>>>(a, 1);
+  else
+    logprob_bwd_kernel<T, 4><<<grid, dim3(256), 0, st>>>(a, chunks);
 }
 
 }  // namespace

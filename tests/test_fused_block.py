@@ -1134,3 +1134,109 @@ def test_gpu_far_offsets():
     y = fused_layer_norm(torch.ones(1 << 17, 1 << 15, dtype=torch.float16,
                                     device="cuda"))
     assert not y[-1].any() and not y[0].any()
+
+
+@pytest.mark.gpu
+def test_gpu_forward_mode_refused():
+    """A tangent is refused, with and without a recorded graph, and not
+    dropped."""
+    from torch.autograd import forward_ad
+    x = torch.randn(4, 16, device="cuda")
+    w = torch.randn(8, 16, device="cuda")
+    t = torch.zeros(4, dtype=torch.int64, device="cuda")
+    for f in (fused_layer_norm, lambda v: fused_linear(v, w),
+              lambda v: fused_linear(x, w, None, None, v @ w.t()),
+              lambda v: token_logprobs(v, t).logprobs):
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(x, torch.ones_like(x))
+            with pytest.raises(RuntimeError, match="jvp"):
+                f(dual)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="jvp"):
+                f(dual)
+
+
+@on_devices
+def test_gradients_have_their_own_memory(device):
+    """Inputs that share one gradient get two tensors, and an input given
+    twice gets the sum."""
+    x, res = (torch.randn(6, 32, device=device, requires_grad=True)
+              for _ in range(2))
+    w = torch.randn(32, 32, device=device)
+    dy = torch.randn(6, 32, device=device)
+    for f in (lambda a, b: sum(fused_layer_norm(a, residual=b)),
+              lambda a, b: fused_linear(a, w, residual=b)):
+        x.grad = res.grad = None
+        f(x, res).backward(dy)
+        assert x.grad.data_ptr() != res.grad.data_ptr()
+        assert dy.data_ptr() not in (x.grad.data_ptr(), res.grad.data_ptr())
+        a, b = x.grad.clone(), res.grad.clone()
+        x.grad.zero_()
+        assert torch.equal(res.grad, b)
+        x.grad = None
+        f(x, x).backward(dy)
+        f2 = x.grad
+        x.grad = res.grad = None
+        same = x.detach().clone().requires_grad_(True)
+        f(x, same).backward(dy)
+        assert torch.equal(f2, x.grad + same.grad)
+        assert a.shape == b.shape
+
+
+# rows that four waves share unevenly; the last size that a wave has alone,
+# and the next
+@on_devices
+@on_types
+@pytest.mark.parametrize("rows", [1, 3, 9])
+@pytest.mark.parametrize("vocab", [3, 255, 1024, 1028, 2048, 2056])
+def test_logprobs_gradient_sizes(device, dtype, rows, vocab):
+    x, t = make_logits(rng(rows, vocab, 5), dtype, device, rows, vocab)
+    run_logprobs(device, x, t, 0)
+
+
+@pytest.mark.gpu
+def test_gpu_two_threads():
+    """Two threads, each on a stream of its own, get the numbers of a pass
+    alone."""
+    import threading
+    torch.manual_seed(6)
+    m = Block(128, 384, 9000).cuda().bfloat16()
+    xs = [torch.randn(r, 128, device="cuda").bfloat16() for r in (3, 200)]
+    ts = [torch.randint(0, 9000, (r,), device="cuda") for r in (3, 200)]
+    want = [step_of(m, x.clone().requires_grad_(True), t)
+            for x, t in zip(xs, ts)]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got[i] = step_of(m, xs[i].clone().requires_grad_(True),
+                                     ts[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join(60)
+    assert not errors and not any(th.is_alive() for th in threads)
+    for g, w in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(g, w))
+
+
+# dbias over few and many rows: one slice, two, and more than are in flight
+@on_devices
+@on_types
+@pytest.mark.parametrize("m", [1, 64, 65, 130, 3001, 9000])
+def test_linear_bias_gradient_rows(device, dtype, m):
+    g = rng(m, 7)
+    x = normal(g, m, 3, dtype=dtype, device=device)
+    w = normal(g, 37, 3, dtype=dtype, device=device)
+    b = torch.zeros(37, device=device, requires_grad=True)
+    dy = normal(g, m, 37, dtype=dtype, device=device)
+    db, = torch.autograd.grad(fused_linear(x, w, b), b, dy)
+    dy = dy.cpu().double()
+    within(db, dy.sum(0), (m + 64) * U * dy.abs().sum(0))
