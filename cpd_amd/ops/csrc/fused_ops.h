@@ -99,10 +99,16 @@ struct GemmArgs {
   const void* res;    // [m, n], row stride res_ld, or null
   long res_ld;
   Act act;
-  float* work;        // gemm_work_floats()
+  float* work;        // gemm_work() floats
+  int tile, slices;   // how it is cut up, by gemm_plan
 };
-// `along`: both operands are
-long gemm_work_floats(long m, long n, long k, Dt dt, bool along);
+// Sets how a product is cut up, from its sizes and layouts.
+void gemm_plan(GemmArgs& g);
+// The same for dx and dW of one layer (A of dx lies along, the rest across);
+// whether one launch for both takes less time than two.
+bool gemm_plan_two(GemmArgs& dx, GemmArgs& dw);
+// The workspace that a planned product needs.
+long gemm_work(const GemmArgs& g);
 constexpr long kMostFeatures = 1L << 22;
 // Whether a 16-bit product takes the operand as it lies (`rows` by k), 16
 // bytes at a time; if not, pad_rows makes a copy that it takes.  Floats are
@@ -112,6 +118,7 @@ bool gemm_few_rows(long m, long n, long k, Dt dt);
 void pad_rows(const void* from, long ld, void* to, long to_ld, int rows,
               int cols, Dt dt, hipStream_t stream);
 void gemm_fused(const GemmArgs& a, hipStream_t stream);
+void gemm_two(const GemmArgs& dx, const GemmArgs& dw, hipStream_t stream);
 
 // dz = dy * act'(z) and the sums of its columns.
 struct ActGradArgs {

@@ -351,14 +351,30 @@ struct Products {
     return {keep.back().const_data_ptr(), ld, across, true};
   }
 
+  // The workspace of a planned product.
+  void give_work(cpd::GemmArgs& g, const Tensor& like) {
+    const long floats = cpd::gemm_work(g);
+    if (!floats) return;
+    keep.push_back(at::empty({floats}, like.options().dtype(at::kFloat)));
+    g.work = keep.back().data_ptr<float>();
+  }
+
   void run(cpd::GemmArgs& g, const Tensor& like) {
-    const long floats = cpd::gemm_work_floats(g.m, g.n, g.k, dt,
-                                              !g.a.across && !g.b.across);
-    if (floats) {
-      keep.push_back(at::empty({floats}, like.options().dtype(at::kFloat)));
-      g.work = keep.back().data_ptr<float>();
-    }
+    cpd::gemm_plan(g);
+    give_work(g, like);
     cpd::gemm_fused(g, st);
+  }
+
+  void run_two(cpd::GemmArgs& dx, cpd::GemmArgs& dw, const Tensor& like) {
+    const bool together = cpd::gemm_plan_two(dx, dw);
+    give_work(dx, like);
+    give_work(dw, like);
+    if (together) {
+      cpd::gemm_two(dx, dw, st);
+    } else {
+      cpd::gemm_fused(dx, st);
+      cpd::gemm_fused(dw, st);
+    }
   }
 };
 
@@ -478,26 +494,30 @@ std::vector<Tensor> linear_bwd(const Tensor& dy, const Tensor& x,
   // dW: dz^T x, the sum runs over m
   Products products{dt, st, {}};
   const bool padded = p.dz != nullptr;
-  cpd::GemmArgs q{};
-  q.dt = q.bias_dt = dt;
-  q.n = (int)k;
-  q.y_ld = k;
+  cpd::GemmArgs q{}, v{};
+  q.dt = q.bias_dt = v.dt = v.bias_dt = dt;
+  q.n = v.n = (int)k;
+  q.y_ld = v.y_ld = k;
   if (need_x) {
     q.a = products.operand(g, false, padded, false, x);
     q.b = products.operand(w, true, false, false, x);
     q.m = (int)m;
     q.k = (int)n;
     q.y = dx.mutable_data_ptr();
-    products.run(q, x);
   }
   if (need_w) {
-    q.a = products.operand(g, true, padded, false, x);
-    q.b = products.operand(r, true, false, false, x);
-    q.m = (int)n;
-    q.k = (int)m;
-    q.y = dw.mutable_data_ptr();
-    products.run(q, x);
+    v.a = products.operand(g, true, padded, false, x);
+    v.b = products.operand(r, true, false, false, x);
+    v.m = (int)n;
+    v.k = (int)m;
+    v.y = dw.mutable_data_ptr();
   }
+  if (need_x && need_w)
+    products.run_two(q, v, x);
+  else if (need_x)
+    products.run(q, x);
+  else if (need_w)
+    products.run(v, x);
   check_launch("linear backward");
   return {dx, dw, db};
 }

@@ -13,6 +13,7 @@
 // bf16 at 8192^3: 1.46 PFLOP/s forward, 1.32 dx, 1.31 dW (the library's plain
 // product: 1.48, 1.39, 1.20); 2048^3: 0.76; floats at 8192 x 2048 x 8192: 0.20.
 #include <type_traits>
+#include <utility>
 
 #include "gemm_tiles.h"
 
@@ -146,13 +147,12 @@ __device__ __forceinline__ void leave_finished(const GemmArgs& g, char* lds,
   });
 }
 
-// The same, or a slice's sums to `part`.
+// The same, or a slice's sums to the workspace.
 template <typename T, int F>
 __device__ __forceinline__ void leave_block(const GemmArgs& g, char* lds,
                                             const f32x4 (*v)[4], int row0,
-                                            int col0, int lane, int slice,
-                                            float* part) {
-  if (!part) {
+                                            int col0, int lane, int slice) {
+  if (g.slices == 1) {
     leave_finished<T, F>(g, lds, v, row0, col0, lane);
     return;
   }
@@ -160,7 +160,7 @@ __device__ __forceinline__ void leave_block(const GemmArgs& g, char* lds,
     row += row0;
     col += col0;
     if (row < g.m && col < g.n)
-      store_some<float, 8>(part + ((long)slice * g.m + row) * g.n + col,
+      store_some<float, 8>(g.work + ((long)slice * g.m + row) * g.n + col,
                            g.n - col, out);
   });
 }
@@ -179,13 +179,11 @@ __device__ __forceinline__ void leave_block(const GemmArgs& g, char* lds,
 // the end of a phase everything but the newest five halves (ten copies a
 // lane) has to have landed, and a copy has more than a tile's time to do so.
 template <typename T, bool AX, bool BX>
-__global__ __launch_bounds__(512, 2) void gemm_256_kernel(GemmArgs g, int tm,
-                                                          int tn) {
-  __shared__ __attribute__((aligned(1024))) char lds[8 * kHalf];
+__device__ __forceinline__ void tile_256(const GemmArgs& g, int id, char* lds) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int bm, bn;
-  tile_of(blockIdx.x, tm, tn, bm, bn);
+  tile_of(id, (g.m + 255) / 256, (g.n + 255) / 256, bm, bn);
   const int m0 = bm * 256, n0 = bn * 256;
   const int wm = (wave >> 2) * 64, wn = (wave & 3) * 32;
   const u32 lds0 = lds_address(lds);
@@ -319,15 +317,13 @@ __global__ __launch_bounds__(512, 2) void gemm_256_kernel(GemmArgs g, int tm,
 // all have read tile t, whose place tile t + 4 takes.  The tiles of k may be
 // shared out over `slices` blocks, whose sums then go to `part` as they are.
 template <typename T, bool AX, bool BX>
-__global__ __launch_bounds__(512, 2) void gemm_128_kernel(GemmArgs g, int tm,
-                                                          int tn, int slices,
-                                                          float* part) {
-  __shared__ __attribute__((aligned(1024))) char lds[8 * kHalf];
+__device__ __forceinline__ void tile_128(const GemmArgs& g, int id, char* lds) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int slice = blockIdx.x / (tm * tn);
+  const int tm = (g.m + 127) / 128, tn = (g.n + 127) / 128, slices = g.slices;
+  const int slice = id / (tm * tn);
   int bm, bn;
-  tile_of(blockIdx.x % (tm * tn), tm, tn, bm, bn);
+  tile_of(id % (tm * tn), tm, tn, bm, bn);
   const int m0 = bm * 128, n0 = bn * 128;
   const int wk = wave >> 2, wm = (wave >> 1 & 1) * 64, wn = (wave & 1) * 64;
   const u32 lds0 = lds_address(lds);
@@ -433,7 +429,7 @@ __global__ __launch_bounds__(512, 2) void gemm_128_kernel(GemmArgs g, int tm,
                       lds + (wave ^ 4) * 8192 + (i * 4 + j) * 1024 + lane * 16);
   __syncthreads();
   leave_block<T, 2>(g, lds + wave * 8192, out, m0 + wm + wk * 32, n0 + wn, lane,
-                 slice, part);
+                    slice);
 }
 
 // 128 by 128 results of floats (gemm_tiles.h), tiles of 32 k.  Waves 4-11 read
@@ -442,17 +438,15 @@ __global__ __launch_bounds__(512, 2) void gemm_128_kernel(GemmArgs g, int tm,
 // the cutting goes on under the matrix instructions (1536 cycles a tile).  With
 // both done by all of eight waves in turn a tile took 1.6 us, with four waves
 // that cut 1.3 us, which was their time.
-constexpr int kFloatThreads = 768;
-
 template <bool AX, bool BX>
-__global__ __launch_bounds__(kFloatThreads, 3) void gemm_float_kernel(
-    GemmArgs g, int tm, int tn, int slices, float* part) {
-  __shared__ __attribute__((aligned(1024))) char lds[12 * kPlane];
+__device__ __forceinline__ void tile_floats(const GemmArgs& g, int id,
+                                            char* lds) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int slice = blockIdx.x / (tm * tn);
+  const int tm = (g.m + 127) / 128, tn = (g.n + 127) / 128, slices = g.slices;
+  const int slice = id / (tm * tn);
   int bm, bn;
-  tile_of(blockIdx.x % (tm * tn), tm, tn, bm, bn);
+  tile_of(id % (tm * tn), tm, tn, bm, bn);
   const int m0 = bm * 128, n0 = bn * 128;
   const int all = (g.k + kFloatK - 1) / kFloatK;
   const int per = (all + slices - 1) / slices;
@@ -524,9 +518,46 @@ __global__ __launch_bounds__(kFloatThreads, 3) void gemm_float_kernel(
   // waves may still be reading it, so each wave leaves through the half of LDS
   // that the last tile is not in, 12 KB a wave: 48 rows, then 16.
   char* free = lds + ((to - from) & 1) * (6 * kPlane) + wave * 12288;
-  leave_block<float, 3>(g, free, acc, m0 + wm, n0 + wn, lane, slice, part);
-  leave_block<float, 1>(g, free, acc + 3, m0 + wm + 48, n0 + wn, lane, slice,
-                        part);
+  leave_block<float, 3>(g, free, acc, m0 + wm, n0 + wn, lane, slice);
+  leave_block<float, 1>(g, free, acc + 3, m0 + wm + 48, n0 + wn, lane, slice);
+}
+
+template <typename T>
+constexpr int kThreads = __is_same(T, float) ? 768 : 512;
+template <typename T>
+constexpr int kLds = __is_same(T, float) ? 12 * kPlane : 8 * kHalf;
+
+template <typename T, bool AX, bool BX, int TILE>
+__device__ __forceinline__ void tile_any(const GemmArgs& g, int id, char* lds) {
+  if constexpr (__is_same(T, float))
+    tile_floats<AX, BX>(g, id, lds);
+  else if constexpr (TILE == 256)
+    tile_256<T, AX, BX>(g, id, lds);
+  else
+    tile_128<T, AX, BX>(g, id, lds);
+}
+
+template <typename T, bool AX, bool BX, int TILE>
+__global__ __launch_bounds__(kThreads<T>, kThreads<T> / 256) void gemm_kernel(
+    GemmArgs g) {
+  __shared__ __attribute__((aligned(1024))) char lds[kLds<T>];
+  tile_any<T, AX, BX, TILE>(g, blockIdx.x, lds);
+}
+
+// dx and dW in one launch, so that neither's last round leaves CUs idle and
+// fewer slices of k fill them: backward of 3000 x 2500 by 2500 bf16 took 131 us
+// in two launches and takes 102, of 512 x 2048 by 1000 floats 56 and 46.  `first`
+// blocks are dx's, or dW's if those take longer.
+template <typename T, int DX, int DW>
+__global__ __launch_bounds__(kThreads<T>, kThreads<T> / 256) void gemm_two_kernel(
+    GemmArgs dx, GemmArgs dw, int first, bool dw_first) {
+  __shared__ __attribute__((aligned(1024))) char lds[kLds<T>];
+  const int id = blockIdx.x;
+  const bool second = id >= first;
+  if (second == dw_first)
+    tile_any<T, false, true, DX>(dx, second ? id - first : id, lds);
+  else
+    tile_any<T, true, true, DW>(dw, second ? id - first : id, lds);
 }
 
 // Few rows of A (16 F), both operands along: bound by reading B once.  A block
@@ -541,8 +572,7 @@ __global__ __launch_bounds__(kFloatThreads, 3) void gemm_float_kernel(
 // and 34, 37, 40 and 50 for W = 2 against 40 of gemm_128_kernel; with 34 MB 11,
 // 12, 16 and 21 against 17; with 8 MB 6, 7, 7 and 9 against 14.
 template <typename T, int F, int W>
-__global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g, int slices,
-                                                        float* part) {
+__global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g) {
   constexpr int VEC = 16 / sizeof(T);    // a lane's elements of a load
   constexpr int UNIT = 128 / sizeof(T);  // k of a line; a lane has two loads
   constexpr int BATCH = F == 1 ? (W == 1 ? 4 : 2) : F == 2 && W == 1 ? 2 : 1;
@@ -553,7 +583,7 @@ __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g, int slices,
   const int slice = blockIdx.x / blocks;
   const int n0 = (blockIdx.x % blocks) * (16 * W);
   const int units = (g.k + UNIT - 1) / UNIT;
-  const int per = (units + slices - 1) / slices;
+  const int per = (units + g.slices - 1) / g.slices;
   const int from = slice * per, to = min(from + per, units);
   const int k0 = (lane >> 4) * 2 * VEC;
   // (rows behind the last one repeat it: their results are not stored)
@@ -644,9 +674,9 @@ __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g, int slices,
     const int row = i / W * 16 + (lane & 15);
     const int col = n0 + i % W * 16 + (lane >> 4) * 4;
     float v[4] = {t[0], t[1], t[2], t[3]}, bias[4] = {};
-    if (part) {
+    if (g.slices > 1) {
       if (row < g.m && col < g.n)
-        store_some<float, 4>(part + ((long)slice * g.m + row) * g.n + col,
+        store_some<float, 4>(g.work + ((long)slice * g.m + row) * g.n + col,
                              g.n - col, v);
       continue;
     }
@@ -657,17 +687,16 @@ __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g, int slices,
 
 // The slices' sums, in order, and what follows the product.
 template <typename T>
-__global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs g, int slices,
-                                                        const float* part) {
+__global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs g) {
   const int chunks = (g.n + 7) / 8;
   const long all = (long)g.m * chunks;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all;
        i += (long)gridDim.x * 256) {
     const int row = (int)(i / chunks), col = (int)(i % chunks) * 8;
     float v[8] = {}, bias[8] = {};
-    for (int s = 0; s < slices; ++s) {
+    for (int s = 0; s < g.slices; ++s) {
       float u[8];
-      load_some<float, 8>(part + ((long)s * g.m + row) * g.n + col, g.n - col, u);
+      load_some<float, 8>(g.work + ((long)s * g.m + row) * g.n + col, g.n - col, u);
 #pragma unroll
       for (int q = 0; q < 8; ++q) v[q] += u[q];
     }
@@ -685,87 +714,103 @@ bool gemm_few_rows(long m, long n, long k, Dt dt) {
 
 namespace {
 
-// How a product is cut up.  The tile kernels have one block a CU, so time goes
-// by rounds of 256 blocks.  In units of a 128-tile's 64 k (0.48 us): a 256-tile's
-// take 2.4, 32 k of floats 2.3, what a block does before and behind its loop 10
-// and 16, and the joining kernel 8 and 8 bytes for each partial sum at 4 TB/s.
+// How a product is cut up, and the time that it takes.  The tile kernels have
+// one block a CU, so time goes by rounds of 256 blocks.  In units of a 128-tile's
+// 64 k (0.48 us): a 256-tile's take 2.4, 32 k of floats 2.3, what a block does
+// before and behind its loop 10 and 16, and the joining kernel 8 and 8 bytes for
+// each partial sum at 4 TB/s.
 struct Plan {
-  int tile;    // 256 or 128; 32 or 16 for gemm_rows_kernel
-  int slices;  // of k, not for 256
+  int tile;      // 256 or 128; 32 or 16 for gemm_rows_kernel
+  int slices;    // of k; 1 for 256
+  long blocks;
+  double block;  // a block's time
+  double join;   // the joining kernel's
 };
 
-Plan plan_for(long m, long n, long k, Dt dt, bool along) {
-  if (m < 1 || n < 1) return {128, 1};  // nothing will be launched
-  if (along && gemm_few_rows(m, n, k, dt)) {
-    // 16 rows of B a block, or 32 where A would be read too often
-    const bool wide = m <= 32 && n * k * dt_size(dt) > (48L << 20);
-    const long blocks = wide ? (n + 31) / 32 : (n + 15) / 16;
-    const long lines = k * dt_size(dt) / 128;
-    long s = 512 / blocks;  // two blocks a CU, eight lines a wave at least
-    if (s > lines / 64) s = lines / 64;
-    return {wide ? 32 : 16, (int)(s < 1 ? 1 : s > 32 ? 32 : s)};
-  }
-  auto count = [&](long t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
-  auto rounds = [](long blocks) { return (double)((blocks + 255) / 256); };
-  const bool floats = dt == Dt::f32;
+Plan plan_of(const GemmArgs& g, int tile, int slices) {
+  const bool floats = g.dt == Dt::f32;
   const long tile_k = floats ? kFloatK : kTileK;
-  const long tiles = (k + tile_k - 1) / tile_k;
-  const double unit = floats ? 2.3 : 1;
-  const long small = count(128);
-  Plan best = {256, 1};
-  double least = floats ? 1e30 : rounds(count(256)) * (2.4 * tiles + 16);
-  for (int s = 1; s <= 32 && (s == 1 || tiles / s >= 4); ++s) {
-    double cost = rounds(small * s) * ((tiles + s - 1) / s * unit + 10);
-    if (s > 1) cost += 8 + s * (double)m * n * 8 / 1.9e6;
-    if (cost < least) {
-      least = cost;
-      best = {128, s};
-    }
-  }
-  return best;
+  const long tiles = (g.k + tile_k - 1) / tile_k;
+  const long tm = (g.m + tile - 1) / tile, tn = (g.n + tile - 1) / tile;
+  const double k = (double)((tiles + slices - 1) / slices);
+  return {tile, slices, tm * tn * slices,
+          tile == 256 ? 2.4 * k + 16 : (floats ? 2.3 : 1) * k + 10,
+          slices > 1 ? 8 + slices * (double)g.m * g.n * 8 / 1.9e6 : 0};
+}
+
+// Calls f with the ways there are; at least four tiles of k a slice.
+template <typename F>
+void each_plan(const GemmArgs& g, bool powers, F f) {
+  if (g.dt != Dt::f32) f(plan_of(g, 256, 1));
+  const long tiles = g.k / (g.dt == Dt::f32 ? kFloatK : kTileK);
+  for (int s = 1; s <= 32 && (s == 1 || tiles / s >= 4); s = powers ? 2 * s : s + 1)
+    f(plan_of(g, 128, s));
+}
+
+double rounds(long blocks) { return (double)((blocks + 255) / 256); }
+
+double time_of(const Plan& p) { return rounds(p.blocks) * p.block + p.join; }
+
+// Blocks of two kinds, the longer ones first, on 256 CUs.
+double time_of_two(Plan a, Plan b) {
+  if (a.block < b.block) std::swap(a, b);
+  const long over = a.blocks % 256;  // CUs that have one of the first kind more
+  const double start = a.blocks / 256 * a.block;
+  const double busy = over ? start + a.block : start;
+  // what the other CUs do of the second kind meanwhile
+  const long turns = over ? (long)(a.block / b.block) : 0;
+  const long done = (256 - over) * turns;
+  const double joins = a.join + b.join;
+  if (over && b.blocks <= done) return busy + joins;
+  const long left = b.blocks - done, last = left % 256;
+  const double free = start + turns * b.block, whole = left / 256 * b.block;
+  const double end = last == 0            ? whole
+                     : last <= 256 - over ? free - busy + whole + b.block
+                                          : whole + b.block;
+  return busy + (end > whole ? end : whole) + joins;
+}
+
+void take(GemmArgs& g, const Plan& p) {
+  g.tile = p.tile;
+  g.slices = p.slices;
+}
+
+unsigned blocks_of(const GemmArgs& g) {
+  const int tm = g.tile < 128 ? 1 : (g.m + g.tile - 1) / g.tile;
+  return (unsigned)(tm * ((g.n + g.tile - 1) / g.tile) * g.slices);
 }
 
 template <typename O>
-void join_slices(const GemmArgs& g, const Plan& p, hipStream_t st) {
+void join_slices(const GemmArgs& g, hipStream_t st) {
+  if (g.slices == 1) return;
   const long blocks = ((long)g.m * ((g.n + 7) / 8) + 255) / 256;
   gemm_join_kernel<O><<<dim3((unsigned)(blocks < 4096 ? blocks : 4096)),
-                        dim3(256), 0, st>>>(g, p.slices, g.work);
+                        dim3(256), 0, st>>>(g);
 }
 
 template <typename T, bool AX, bool BX>
 void gemm_tiles_t(const GemmArgs& g, hipStream_t st) {
-  const Plan p = plan_for(g.m, g.n, g.k, g.dt, !g.a.across && !g.b.across);
-  const int tm = (g.m + p.tile - 1) / p.tile, tn = (g.n + p.tile - 1) / p.tile;
-  float* part = p.slices > 1 ? g.work : nullptr;
-  const dim3 grid(tm * tn * p.slices);
-  if constexpr (!AX && !BX) {
-    if (p.tile < 128) {
-      const dim3 grid(tn * p.slices);
-      auto start = [&](auto f, auto w) {
-        gemm_rows_kernel<T, decltype(f)::value, decltype(w)::value>
-            <<<grid, dim3(512), 0, st>>>(g, p.slices, part);
-      };
-      using std::integral_constant;
-      const integral_constant<int, 1> one;
-      const integral_constant<int, 2> two;
-      const integral_constant<int, 4> four;
-      if (p.tile == 32)
-        g.m <= 16 ? start(one, two) : start(two, two);
-      else
-        g.m <= 16 ? start(one, one) : g.m <= 32 ? start(two, one) : start(four, one);
-      if (part) join_slices<T>(g, p, st);
-      return;
-    }
+  const dim3 grid(blocks_of(g)), threads(kThreads<T>);
+  if (g.tile == 256) {
+    if constexpr (!__is_same(T, float))
+      gemm_kernel<T, AX, BX, 256><<<grid, threads, 0, st>>>(g);
+  } else if (g.tile == 128) {
+    gemm_kernel<T, AX, BX, 128><<<grid, threads, 0, st>>>(g);
+  } else if constexpr (!AX && !BX) {
+    auto start = [&](auto f, auto w) {
+      gemm_rows_kernel<T, decltype(f)::value, decltype(w)::value>
+          <<<grid, dim3(512), 0, st>>>(g);
+    };
+    using std::integral_constant;
+    const integral_constant<int, 1> one;
+    const integral_constant<int, 2> two;
+    const integral_constant<int, 4> four;
+    if (g.tile == 32)
+      g.m <= 16 ? start(one, two) : start(two, two);
+    else
+      g.m <= 16 ? start(one, one) : g.m <= 32 ? start(two, one) : start(four, one);
   }
-  if constexpr (__is_same(T, float))
-    gemm_float_kernel<AX, BX><<<grid, dim3(kFloatThreads), 0, st>>>(
-        g, tm, tn, p.slices, part);
-  else if (p.tile == 256)
-    gemm_256_kernel<T, AX, BX><<<grid, dim3(512), 0, st>>>(g, tm, tn);
-  else
-    gemm_128_kernel<T, AX, BX><<<grid, dim3(512), 0, st>>>(g, tm, tn, p.slices,
-                                                           part);
-  if (part) join_slices<T>(g, p, st);
+  join_slices<T>(g, st);
 }
 
 template <typename T>
@@ -776,6 +821,29 @@ void gemm_tiles(const GemmArgs& g, hipStream_t st) {
     gemm_tiles_t<T, false, true>(g, st);
   else
     gemm_tiles_t<T, true, true>(g, st);
+}
+
+template <typename T>
+void gemm_two_tiles(const GemmArgs& dx, const GemmArgs& dw, hipStream_t st) {
+  const bool dw_first = plan_of(dw, dw.tile, dw.slices).block >
+                        plan_of(dx, dx.tile, dx.slices).block;
+  const unsigned nx = blocks_of(dx), nw = blocks_of(dw);
+  const dim3 grid(nx + nw), threads(kThreads<T>);
+  const int first = (int)(dw_first ? nw : nx);
+  if constexpr (__is_same(T, float)) {
+    gemm_two_kernel<T, 128, 128><<<grid, threads, 0, st>>>(dx, dw, first, dw_first);
+  } else {
+    if (dx.tile == 256 && dw.tile == 256)
+      gemm_two_kernel<T, 256, 256><<<grid, threads, 0, st>>>(dx, dw, first, dw_first);
+    else if (dx.tile == 256)
+      gemm_two_kernel<T, 256, 128><<<grid, threads, 0, st>>>(dx, dw, first, dw_first);
+    else if (dw.tile == 256)
+      gemm_two_kernel<T, 128, 256><<<grid, threads, 0, st>>>(dx, dw, first, dw_first);
+    else
+      gemm_two_kernel<T, 128, 128><<<grid, threads, 0, st>>>(dx, dw, first, dw_first);
+  }
+  join_slices<T>(dx, st);
+  join_slices<T>(dw, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -873,9 +941,62 @@ void gemm_fused(const GemmArgs& g, hipStream_t st) {
     gemm_tiles<f16_t>(g, st);
 }
 
-long gemm_work_floats(long m, long n, long k, Dt dt, bool along) {
-  const Plan p = plan_for(m, n, k, dt, along);
-  return p.slices > 1 ? p.slices * m * n : 0;
+void gemm_two(const GemmArgs& dx, const GemmArgs& dw, hipStream_t st) {
+  if (dx.dt == Dt::f32)
+    gemm_two_tiles<float>(dx, dw, st);
+  else if (dx.dt == Dt::bf16)
+    gemm_two_tiles<bf16_t>(dx, dw, st);
+  else
+    gemm_two_tiles<f16_t>(dx, dw, st);
+}
+
+void gemm_plan(GemmArgs& g) {
+  g.tile = 128;
+  g.slices = 1;
+  if (g.m < 1 || g.n < 1) return;  // nothing will be launched
+  if (!g.a.across && !g.b.across && gemm_few_rows(g.m, g.n, g.k, g.dt)) {
+    // 16 rows of B a block, or 32 where A would be read too often
+    const long bytes = (long)g.n * g.k * dt_size(g.dt);
+    g.tile = g.m <= 32 && bytes > (48L << 20) ? 32 : 16;
+    const long blocks = (g.n + g.tile - 1) / g.tile;
+    const long lines = (long)g.k * dt_size(g.dt) / 128;
+    long s = 512 / blocks;  // two blocks a CU, eight lines a wave at least
+    if (s > lines / 64) s = lines / 64;
+    g.slices = (int)(s < 1 ? 1 : s > 32 ? 32 : s);
+  } else {
+    double least = INFINITY;
+    each_plan(g, false, [&](const Plan& p) {
+      if (time_of(p) >= least) return;
+      least = time_of(p);
+      take(g, p);
+    });
+  }
+}
+
+bool gemm_plan_two(GemmArgs& a, GemmArgs& b) {
+  gemm_plan(a);
+  gemm_plan(b);
+  // (where both fill their rounds two launches are not slower: 2048^3 of bf16
+  // took 45 us in two, 48 in one)
+  double least = time_of(plan_of(a, a.tile, a.slices)) +
+                 time_of(plan_of(b, b.tile, b.slices));
+  bool together = false;
+  each_plan(a, true, [&](const Plan& p) {
+    each_plan(b, true, [&](const Plan& q) {
+      const double time = time_of_two(p, q);
+      // (a launch holds less than 2^32 threads)
+      if (time >= least || p.blocks + q.blocks > 1L << 22) return;
+      least = time;
+      together = true;
+      take(a, p);
+      take(b, q);
+    });
+  });
+  return together;
+}
+
+long gemm_work(const GemmArgs& g) {
+  return g.slices > 1 ? (long)g.slices * g.m * g.n : 0;
 }
 
 bool gemm_takes(const Operand& o, long rows) {
