@@ -14,20 +14,24 @@
 // 32-bit floats around the largest value seen so far; S and A are rescaled
 // when that grows, so any logits' range is safe.
 //
-// The alternatives ride along: each wave holds the best 64 of what it has
-// read as a sorted list, one entry a lane, and compares a whole vector of
-// new values with the k-th entry before it does anything else.  For values in
-// no order that test fails about k log(n / k) times in n values; values that
-// keep rising pass one and all, which is slower but as right.
+// The alternatives ride along.  Each wave holds the best 64 of what it has read
+// as a sorted list, one entry a lane, and a bar below which nothing need be
+// kept: the k-th entry, and at a row's start the k-th largest of the lanes'
+// maxima.  What passes is put aside in LDS, and a few of those at a time are
+// sorted and joined.  For values in no order the bar is passed about
+// k log(n / k) times in n values; values that keep rising pass often, which is
+// slower but as right.
 //
 // Without alternatives 4096 rows of 50021 bf16 take 95 us (4.3 TB/s) forward and
-// 149 backward (5.5 TB/s).  Alternatives add the work of inserting them: 2048
-// rows of 131072 fp16 take 104 us, 123 with one, 154 with five, 195 with
-// sixteen, 305 with 64.
+// 149 backward (5.5 TB/s).  Alternatives add work: 2048 rows of 131072 fp16 take
+// 99 us, 121 with one, 143 with five, 169 with sixteen, 224 with 64 (inserted one
+// by one 123, 154, 195 and 305).
 //
 // A row of -inf alone has log probability -inf, entropy 0 and no gradient.
 // NaN or +inf in a row makes its log probabilities NaN; among the
 // alternatives NaN counts as the largest.
+#include <type_traits>
+
 #include "fused_ops.h"
 
 namespace cpd {
@@ -45,6 +49,14 @@ __device__ __forceinline__ float fast_exp(float x) {  // e^x, e^-inf = 0
 // A distance from the maximum, kept finite: below this e^d is zero, and zero
 // times an overflowed distance would be NaN.
 __device__ __forceinline__ float near(float d) { return fmaxf(d, -1e4f); }
+
+// (By its bits: of bf16 values taken as floats the compiler makes a maximum of
+// bf16, which the machine does not have.)
+__device__ __forceinline__ float as_float(float x) { return x; }
+__device__ __forceinline__ float as_float(f16_t x) { return (float)x; }
+__device__ __forceinline__ float as_float(bf16_t x) {
+  return __uint_as_float((u32)__builtin_bit_cast(unsigned short, x) << 16);
+}
 
 struct Soft {  // running maximum and sums
   float m, s, a;
@@ -93,74 +105,111 @@ __device__ __forceinline__ u64 lane_key(u64 v, int lane) {
   return ((u64)hi << 32) | lo;
 }
 
-__device__ __forceinline__ u64 key_across(u64 v, int d) {
-  const u32 lo = __shfl_xor((u32)v, d, 64), hi = __shfl_xor((u32)(v >> 32), d, 64);
-  return ((u64)hi << 32) | lo;
+// v of lane ^ D, within the instruction (a shuffle through LDS takes ten times
+// as long).
+template <int D>
+__device__ __forceinline__ u32 across(u32 v) {
+  auto dpp = [](u32 x, auto ctrl) {
+    return (u32)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf,
+                                            0xf, true);
+  };
+  using std::integral_constant;
+  if constexpr (D == 1) return dpp(v, integral_constant<int, 0xB1>());
+  if constexpr (D == 2) return dpp(v, integral_constant<int, 0x4E>());
+  if constexpr (D == 4)  // 7, and 3 of it back
+    return dpp(dpp(v, integral_constant<int, 0x141>()), integral_constant<int, 0x1B>());
+  if constexpr (D == 8) return dpp(v, integral_constant<int, 0x128>());
+  if constexpr (D == 15) return dpp(v, integral_constant<int, 0x140>());
+  if constexpr (D == 16) {
+    const auto both = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? both[0] : both[1];
+  }
+  if constexpr (D == 32) {
+    const auto both = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? both[0] : both[1];
+  }
+  if constexpr (D == 63) return across<32>(across<16>(across<15>(v)));
+}
+
+template <int D>
+__device__ __forceinline__ u64 key_across(u64 v) {
+  return ((u64)across<D>((u32)(v >> 32)) << 32) | across<D>((u32)v);
 }
 
 // The larger of two lanes' keys, or the smaller, to each its own.
-__device__ __forceinline__ u64 exchange(u64 key, int d, bool larger) {
-  const u64 other = key_across(key, d);
+template <int D>
+__device__ __forceinline__ u64 exchange(u64 key, bool larger) {
+  const u64 other = key_across<D>(key);
   return (other > key) == larger ? other : key;
+}
+
+// Keys that rise and fall once (in groups of 2 D lanes) into order.
+template <int D>
+__device__ __forceinline__ u64 merge(u64 key, int lane, bool falling) {
+  key = exchange<D>(key, !(lane & D) == falling);
+  if constexpr (D > 1) key = merge<D / 2>(key, lane, falling);
+  return key;
+}
+
+// A wave's keys in order, the largest first; those behind the n-th are 0.
+template <int SIZE = 2>
+__device__ __forceinline__ u64 sort(u64 key, int lane, int n) {
+  key = merge<SIZE / 2>(key, lane, !(lane & SIZE));
+  if constexpr (SIZE < 64)
+    if (n > SIZE) key = sort<SIZE * 2>(key, lane, n);
+  return key;
 }
 
 // The wave's list: lane i holds the i-th entry.
 struct Top {
-  u64 mine, least;  // this lane's entry; the k-th entry
-  int lane, k;
+  u64 mine;
+  int lane;
 
-  __device__ __forceinline__ void start(int k_) {
-    mine = least = 0;
+  __device__ __forceinline__ void start() {
+    mine = 0;
     lane = threadIdx.x & 63;
-    k = k_;
-  }
-  // what a value has to pass, NaN until there are k entries
-  __device__ __forceinline__ float bar() const {
-    return least ? key_value(least) : NAN;
   }
   // Joins a list in order, the largest first, one key a lane.
   __device__ __forceinline__ void join_list(u64 key) {
     // the larger of the i-th and the other's i-th from its end: the 64 best,
-    // rising and falling once, which six exchanges put in order
-    const u64 back = key_across(key, 63);
-    mine = back > mine ? back : mine;
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) mine = exchange(mine, d, !(lane & d));
-    least = lane_key(mine, k - 1);
+    // rising and falling once
+    const u64 back = key_across<63>(key);
+    mine = merge<32>(back > mine ? back : mine, lane, true);
   }
-  __device__ __forceinline__ void insert(u64 key) {
-    const int at = __popcll(__ballot(mine > key));
-    // the entry of the lane below (wave_shr:1)
-    const u32 lo = __builtin_amdgcn_update_dpp(0, (int)(u32)mine, 0x138, 0xf,
-                                               0xf, false);
-    const u32 hi = __builtin_amdgcn_update_dpp(0, (int)(u32)(mine >> 32),
-                                               0x138, 0xf, 0xf, false);
-    const u64 below = ((u64)hi << 32) | lo;
-    mine = lane < at ? mine : lane == at ? key : below;
-    least = lane_key(mine, k - 1);
-  }
-  // Every lane's key, the best ones kept: a few are inserted one by one, many
-  // are put in order together (21 exchanges) and joined.  (For a list of one or
-  // two few of the many would be inserted.)
-  __device__ __forceinline__ void offer(u64 key) {
-    u64 mask = __ballot(key > least);
-    if (__popcll(mask) > 24 && k > 2) {
-      key = key > least ? key : 0;
-#pragma unroll 1
-      for (int size = 2; size <= 64; size *= 2)
-#pragma unroll 1
-        for (int d = size / 2; d > 0; d >>= 1)
-          key = exchange(key, d, !(lane & d) == !(lane & size));
-      join_list(key);
-      return;
-    }
-    while (mask) {
-      const int from = __ffsll(mask) - 1;
-      insert(lane_key(key, from));
-      if (lane == from) key = 0;
-      mask = __ballot(key > least);
-    }
-  }
+};
+
+// The smallest float above x (infinity for infinity).
+__device__ __forceinline__ float above(float x) {
+  const u32 u = __float_as_uint(x);
+  return x == INFINITY ? x
+         : x == 0.f    ? __uint_as_float(1)
+                       : __uint_as_float(u >> 31 ? u - 1 : u + 1);
+}
+
+__device__ __forceinline__ float uniform(float x) {
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x)));
+}
+
+// Floats that rise and fall once into order, and any 64 into falling order.
+template <int D>
+__device__ __forceinline__ float merge_floats(float x, int lane, bool falling) {
+  const float y = __uint_as_float(across<D>(__float_as_uint(x)));
+  x = !(lane & D) == falling ? fmaxf(x, y) : fminf(x, y);
+  if constexpr (D > 1) x = merge_floats<D / 2>(x, lane, falling);
+  return x;
+}
+template <int SIZE = 2>
+__device__ __forceinline__ float sort_floats(float x, int lane) {
+  x = merge_floats<SIZE / 2>(x, lane, !(lane & SIZE));
+  if constexpr (SIZE < 64) x = sort_floats<SIZE * 2>(x, lane);
+  return x;
+}
+
+// What a wave has found for its list and not put there yet.  Less than 64 wait
+// from one vector to the next, each of which may add all of its elements.
+template <int VEC>
+struct Pending {
+  u64 key[64 + 64 * VEC];
 };
 
 // What one part of a row gives, for the joining kernel.
@@ -237,65 +286,16 @@ __device__ __forceinline__ void block_join(Soft& v, Top& top, Soft* softs,
   }
 }
 
-struct Found {
-  float value[64][4];  // 16 bytes of T
-  int at[64], done[64];
-};
-
-// Offers a wave's vectors, one a lane, the first of them from index `from` on.
-// (Rare, so it is kept small: it works through LDS and in loops, and hides its
-// lane number from the compiler, which otherwise works out everything that
-// depends on it ahead of the row and holds it in 80 registers.)
-template <typename T>
-__device__ __forceinline__ void search(Top& top,
-                                       const typename Vec16<T>::type* seen,
-                                       Found& found, bool odd, int from, int to) {
-  constexpr int VEC = Vec16<T>::N;
-  asm volatile("" : "+v"(top.lane));
-  const typename Vec16<T>::type u = seen[top.lane];
-  const int at = from + top.lane * VEC;
-  // the largest value, where it is first, and the next one
-  float most = -INFINITY, second = -INFINITY;
-  int done = -1;
-#pragma unroll
-  for (int i = VEC - 1; i >= 0; --i) {
-    const float y = (float)u[i];
-    if (y >= most) {
-      second = done >= 0 ? most : second;
-      most = y;
-      done = i;
-    } else {
-      second = fmaxf(second, y);
-    }
-  }
-  bool mine = odd || !(most <= top.bar());
-  u64 mask = __ballot(mine);
-  if (!mask) return;
-  if (__popcll(mask) > 8 && !__ballot(odd)) {
-    // Many pass, as at a row's start: their largest values first, after which
-    // most of the others do not.  (One that equals the bar may come before
-    // what set it here.)
-    top.offer(mine && at + done < to ? key_of(most, at + done) : 0);
-    mine = mine && !(second < top.bar());
-    mask = __ballot(mine);
-    if (!mask) return;
-  } else {
-    done = -1;
-  }
-  // the vectors that are left side by side, and from there one value a lane
-  const int rank = __popcll(mask & ((1ull << top.lane) - 1));
-  if (mine) {
-    *reinterpret_cast<typename Vec16<T>::type*>(found.value[rank]) = u;
-    found.at[rank] = at;
-    found.done[rank] = done;
-  }
+// Joins the `count` pending keys, 64 at a time.
+template <int VEC>
+__device__ __forceinline__ void settle(Top& top, Pending<VEC>& pending, int& count) {
   __builtin_amdgcn_wave_barrier();
-  const int many = __popcll(mask) * VEC;
-  for (int i = top.lane; i - top.lane < many; i += 64) {
-    const int slot = i / VEC & 63, index = found.at[slot] + i % VEC;
-    const bool in = i < many && index < to && found.done[slot] != i % VEC;
-    const float value = (float)reinterpret_cast<const T*>(found.value)[i & (64 * VEC - 1)];
-    top.offer(in ? key_of(value, index) : 0);
+#pragma unroll 1
+  while (count > 0) {
+    const int n = count < 64 ? count : 64;
+    count -= n;
+    const u64 key = top.lane < n ? pending.key[count + top.lane] : 0;
+    top.join_list(sort(key, top.lane, n));
   }
   __builtin_amdgcn_wave_barrier();
 }
@@ -306,17 +306,23 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int parts,
                                                       u64* keys) {
   constexpr int VEC = Vec16<T>::N;
   constexpr int TPR = WAVES * 64;
-  // (with alternatives 16-bit rows have registers for two: with four and 138
-  // registers 16384 rows of 8192 with five of them took 225 us instead of 196)
+  // vectors a lane that are worked on together (with alternatives 16-bit rows have
+  // registers for two: with four 16384 rows of 8192 with five of them took 182 us
+  // instead of 161)
   constexpr int LOADS = TOP && sizeof(T) == 2 ? 2 : 4;
+  constexpr int STEP = TPR * VEC * LOADS;
+  typedef typename Vec16<T>::type V;
   __shared__ Soft softs[WAVES];
   __shared__ u64 lists[TOP && WAVES > 1 ? WAVES : 1][kMostTop];
-  __shared__ typename Vec16<T>::type seen[TOP ? 4 : 1][LOADS][64];
-  __shared__ Found found[TOP ? 4 : 1];
+  __shared__ Pending<VEC> pendings[TOP ? 4 : 1];
   // (in a scalar register: what a row or a wave shares stays out of the others)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tid = threadIdx.x % TPR;
   const long jobs = a.rows * parts;
+  // (Pending keys do not raise the bar, and joining a few costs half of joining
+  // 64: with one alternative 131072 fp16 took 125 us if four were waited for, 123
+  // if two, 158 if 64; with sixteen 174, 169 and 171.)
+  const int most = min(64, 2 * a.top);
   Top top;
   for (long job0 = (long)blockIdx.x * (256 / TPR); job0 < jobs;
        job0 += (long)gridDim.x * (256 / TPR)) {
@@ -324,7 +330,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int parts,
     if (job >= jobs) break;  // WAVES == 1 only: a whole wave leaves
     const long row = job / parts;
     const int64_t target = a.targets[row];
-    top.start(TOP ? a.top : 1);
+    top.start();
     if (target == a.ignore) {
       if (job == row * parts && tid < 64) {
         if (tid == 0) {
@@ -344,25 +350,18 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int parts,
     const int to = a.vocab - from < per ? a.vocab : from + per;
     const T* x = static_cast<const T*>(a.x) + row * a.ld;
     Soft v = {-INFINITY, 0.f, 0.f};
-    // a few loads a thread at a time, one rescaling for all of them
-    for (int base = from; base < to; base += TPR * VEC * LOADS) {
-      typename Vec16<T>::type u[LOADS];
-      if (base + TPR * VEC * LOADS <= to) {
-#pragma unroll
-        for (int c = 0; c < LOADS; ++c)
-          u[c] = load_raw<T>(x + base + (c * TPR + tid) * VEC, VEC);
-      } else {
-#pragma unroll
-        for (int c = 0; c < LOADS; ++c) {
-          const int at = base + (c * TPR + tid) * VEC;
-          u[c] = load_raw<T>(x + at, to - at, (T)-INFINITY);
-        }
-      }
-      float big = (float)u[0][0];
+    // Values below `bar` need not be kept.  (k of them are from it on, and those
+    // of this wave's that equal it and come later come after them.)
+    float bar = -INFINITY;
+    int count = 0;  // of pending keys
+    bool full = false;  // k of them are NaN: nothing comes before those
+    // one rescaling for a few vectors
+    auto work = [&](int base, const V (&u)[LOADS]) {
+      float big = as_float(u[0][0]);
 #pragma unroll
       for (int c = 0; c < LOADS; ++c)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) big = fmaxf(big, (float)u[c][i]);
+        for (int i = 0; i < VEC; ++i) big = fmaxf(big, as_float(u[c][i]));
       if (big > v.m) {
         const float d = v.m == -INFINITY ? 0.f : near(v.m - big);
         const float f = v.m == -INFINITY ? 0.f : fast_exp(d);
@@ -375,25 +374,80 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int parts,
       for (int c = 0; c < LOADS; ++c)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          const float d = (float)u[c][i] - about;
+          const float d = as_float(u[c][i]) - about;
           const float e = fast_exp(d);
           v.s += e;
           v.a += e * near(d);
         }
-      if (TOP) {
-        // a NaN is passed over by the maximum, but it makes the sum one
-        const bool odd = v.s != v.s;
-        // Values equal to the bar come after what set it and do not pass.
-        if (__ballot(odd || !(big <= top.bar()))) {
-#pragma unroll
-          for (int c = 0; c < LOADS; ++c) seen[wave][c][top.lane] = u[c];
+      if (!TOP) return;
+      // a NaN is passed over by the maximum, but it makes the sum one
+      const bool odd = v.s != v.s;
+      const u64 some = __ballot(odd || !(big < bar));
+      if (!some || full) return;
+      // (What follows is rare.  The lane number and the values are hidden from the
+      // compiler, which otherwise holds all that depends on them in registers
+      // through the whole loop.)
+      int lane = top.lane;
+      asm volatile("" : "+v"(lane));
+      Pending<VEC>& pending = pendings[wave];
+      float now = bar;
+      if (__popcll(some) > 16) {
+        // Many pass, as at a row's start: the k-th of the lanes' maxima is a
+        // better bar, and the next values have to be above it.
+        const float kth = lane_value(sort_floats(fmaxf(big, -INFINITY), lane),
+                                     a.top - 1);
+        now = uniform(fmaxf(now, kth));
+        bar = uniform(fmaxf(bar, above(kth)));
+      }
 #pragma unroll 1
-          for (int c = 0; c < LOADS; ++c)
-            search<T>(top, seen[wave][c], found[wave], odd,
-                      base + (c * TPR + tid - top.lane) * VEC, to);
+      for (int c = 0; c < LOADS; ++c) {
+        typedef u32 Raw __attribute__((ext_vector_type(4)));
+        Raw raw = __builtin_bit_cast(Raw, u[0]);
+#pragma unroll
+        for (int j = 1; j < LOADS; ++j)
+          if (c == j) raw = __builtin_bit_cast(Raw, u[j]);
+        int at = base + (c * TPR + tid - top.lane + lane) * VEC;
+        asm volatile("" : "+v"(raw), "+v"(at));
+        const V w = __builtin_bit_cast(V, raw);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float y = as_float(w[i]);
+          const bool in = !(y < now) && at + i < to;
+          const u64 mask = __ballot(in);
+          if (!mask) continue;
+          if (in)
+            pending.key[count + __builtin_amdgcn_mbcnt_hi(
+                                    (u32)(mask >> 32),
+                                    __builtin_amdgcn_mbcnt_lo((u32)mask, 0))] =
+                key_of(y, at + i);
+          count += __popcll(mask);
+        }
+        if (count < most) continue;
+        settle(top, pending, count);
+        const u64 least = lane_key(top.mine, a.top - 1);
+        if (!least) continue;
+        const float kth = key_value(least);
+        full = kth != kth;
+        now = uniform(fmaxf(now, kth));
+        bar = uniform(fmaxf(bar, above(kth)));
+      }
+    };
+    for (int base = from; base < to; base += STEP) {
+      V u[LOADS];
+      if (base + STEP <= to) {
+#pragma unroll
+        for (int c = 0; c < LOADS; ++c)
+          u[c] = load_raw<T>(x + base + (c * TPR + tid) * VEC, VEC);
+      } else {
+#pragma unroll
+        for (int c = 0; c < LOADS; ++c) {
+          const int at = base + (c * TPR + tid) * VEC;
+          u[c] = load_raw<T>(x + at, to - at, (T)-INFINITY);
         }
       }
+      work(base, u);
     }
+    if (TOP) settle(top, pendings[wave], count);
     v = wave_join(v);
     if (WAVES > 1) block_join<WAVES, TOP>(v, top, softs, lists);
     if (tid < 64) {
@@ -417,7 +471,7 @@ __global__ __launch_bounds__(256) void logprob_join_kernel(
   const int64_t target = a.targets[row];
   if (target == a.ignore) return;  // written by the kernel before
   Top top;
-  top.start(TOP ? a.top : 1);
+  top.start();
   const int wave = threadIdx.x >> 6;
   Soft v = {-INFINITY, 0.f, 0.f};
   const int mine = wave + 4 * top.lane;  // this lane's part: at most 64 parts

@@ -1240,3 +1240,44 @@ def test_linear_bias_gradient_rows(device, dtype, m):
     db, = torch.autograd.grad(fused_linear(x, w, b), b, dy)
     dy = dy.cpu().double()
     within(db, dy.sum(0), (m + 64) * U * dy.abs().sum(0))
+
+
+# What a row's waves tell each other: rows that rise, fall, lie flat, or have
+# all of their largest values in one wave's share, with equal values on both
+# sides of every share's edge.
+@on_devices
+@on_types
+@pytest.mark.parametrize("top_k", [1, 4, 5, 16, 64])
+@pytest.mark.parametrize("vocab", [2100, 20000])
+def test_logprobs_top_orders(device, dtype, top_k, vocab):
+    i = torch.arange(vocab, dtype=torch.float64)
+    g = rng(vocab, top_k)
+    rows = torch.stack([
+        i / vocab, -i / vocab, torch.zeros(vocab), (i % 7) / 8,
+        (i // 512 % 4 == 2).double(), (i // 512 % 4 == 0) * (i % 512),
+        (i // 64 % 3 == 1).double() - (i % 2), -(i // 100),
+        torch.where(i < vocab - 3, -math.inf, 1.0),
+        torch.where(i % 700 == 5, 3.0, -math.inf),
+        torch.randint(0, 3, (vocab,), generator=g).double()])
+    x = rows.to(dtype)
+    t = torch.full((len(x),), 3)
+    out = token_logprobs(x.to(device), t.to(device), top_k)
+    ids = torch.sort(x.double(), dim=-1, descending=True, stable=True)[1][
+        :, :top_k]
+    assert torch.equal(out.top_ids.cpu(), ids)
+
+
+@pytest.mark.gpu
+def test_gpu_logprobs_top_many_rows():
+    """More rows than blocks: what a block kept of one row must not reach the
+    next one that it takes, whose values are smaller."""
+    rows, vocab, last = (1 << 20) + 40, 2056, 40
+    x = torch.full((rows, vocab), 50.0, dtype=torch.float16, device="cuda")
+    x[:last] += torch.arange(vocab, device="cuda") / 128
+    x[-last:] = torch.randn(last, vocab, device="cuda").half()
+    t = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    out = token_logprobs(x, t, 20)
+    for at in (slice(0, last), slice(rows - last, rows)):
+        want = torch.sort(x[at].double(), dim=-1, descending=True,
+                          stable=True)[1][:, :20]
+        assert torch.equal(out.top_ids[at], want)
