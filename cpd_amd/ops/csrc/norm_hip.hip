@@ -28,13 +28,17 @@ struct Shape {
   int tpr, ch;
 };
 
-Shape shape_for(int cols, Dt dt) {
+Shape shape_for(int cols, Dt dt, int most) {
   const int vec = 16 / dt_size(dt);
   const int n = (cols + vec - 1) / vec;
   const int tprs[4] = {16, 64, 256, 1024};
   for (int t : tprs)
-    if (n <= t * 4) return {t, n <= t ? 1 : n <= 2 * t ? 2 : 4};
+    if (n <= t * most) return {t, n <= t ? 1 : n <= 2 * t ? 2 : 4};
   return {0, 0};
+}
+Shape forward_shape(int cols, Dt dt) { return shape_for(cols, dt, 4); }
+Shape backward_shape(int cols, Dt dt) {
+  return shape_for(cols, dt, dt == Dt::f32 ? 4 : 2);
 }
 
 template <typename T, int TPR, int CH>
@@ -182,7 +186,7 @@ __global__ __launch_bounds__(1024) void norm_fwd_loop_kernel(NormArgs a) {
 // ordered before this one is worked on, since the two sums over the row leave
 // memory idle otherwise.  The blocks' shares go to `partial` and are added in a
 // fixed order: no atomics.
-template <typename T, int TPR, int CH>
+template <typename T, int TPR, int CH, bool DS>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_bwd_kernel(
     NormGradArgs a) {
   constexpr int VEC = Vec16<T>::N;
@@ -191,7 +195,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_bwd_kernel(
   const int lane = threadIdx.x % TPR;
   const long stride = (long)gridDim.x * ROWS;
   struct Row {
-    typename Vec16<T>::type s[CH], dy[CH], ds[CH];
+    typename Vec16<T>::type s[CH], dy[CH], ds[DS ? CH : 1];
     float mean, rstd;
   };
   auto fetch = [&](long row, Row& r) {
@@ -204,8 +208,8 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_bwd_kernel(
       r.s[c] = load_raw<T>(static_cast<const T*>(a.s) + row * a.s_ld + at, left);
       r.dy[c] = load_raw<T>(static_cast<const T*>(a.dy) + row * a.dy_ld + at,
                             a.dy ? left : 0);
-      r.ds[c] = load_raw<T>(static_cast<const T*>(a.ds) + row * a.ds_ld + at,
-                            a.ds ? left : 0);
+      if constexpr (DS)
+        r.ds[c] = load_raw<T>(static_cast<const T*>(a.ds) + row * a.ds_ld + at, left);
     }
   };
   float dw[CH][VEC] = {}, db[CH][VEC] = {};
@@ -243,20 +247,29 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_bwd_kernel(
       float o[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
-        o[i] = (float)r.ds[c][i] + r.rstd * (g[c][i] - sg - h[c][i] * sgh);
+        o[i] = r.rstd * (g[c][i] - sg - h[c][i] * sgh) +
+               (DS ? (float)r.ds[DS ? c : 0][i] : 0.f);
       store_vec<T>(dx + at, a.cols - at, o);
     }
   };
-  Row r0, r1;
   const long first = (long)blockIdx.x * ROWS;
   const int mine = threadIdx.x / TPR;
-  fetch(first + mine, r0);
-  for (long row = first; row < a.rows; row += 2 * stride) {
-    fetch(row + stride + mine, r1);
-    work(row + mine, r0);
-    if (row + stride >= a.rows) break;
-    fetch(row + 2 * stride + mine, r0);
-    work(row + stride + mine, r1);
+  if constexpr (TPR == 1024) {
+    for (long row = first; row < a.rows; row += stride) {
+      Row r;
+      fetch(row + mine, r);
+      work(row + mine, r);
+    }
+  } else {
+    Row r0, r1;
+    fetch(first + mine, r0);
+    for (long row = first; row < a.rows; row += 2 * stride) {
+      fetch(row + stride + mine, r1);
+      work(row + mine, r0);
+      if (row + stride >= a.rows) break;
+      fetch(row + 2 * stride + mine, r0);
+      work(row + stride + mine, r1);
+    }
   }
   if (!a.partial) return;
   float* part = a.partial + (long)blockIdx.x * 2 * a.cols;
@@ -388,7 +401,7 @@ __global__ __launch_bounds__(1024) void norm_bwd_join_kernel(
 
 template <typename T>
 void forward_t(const NormArgs& a, hipStream_t st) {
-  const Shape s = shape_for(a.cols, a.dt);
+  const Shape s = forward_shape(a.cols, a.dt);
   if (s.tpr == 0) {
     norm_fwd_loop_kernel<T><<<dim3(a.rows), dim3(1024), 0, st>>>(a);
     return;
@@ -410,9 +423,9 @@ void forward_t(const NormArgs& a, hipStream_t st) {
 #undef CPD_NORM
 }
 
-template <typename T>
+template <typename T, bool DS>
 void backward_t(const NormGradArgs& a, hipStream_t st) {
-  const Shape s = shape_for(a.cols, a.dt);
+  const Shape s = backward_shape(a.cols, a.dt);
   const int blocks = norm_grad_blocks(a.rows, a.cols, a.dt);
   if (s.tpr == 0) {
     norm_bwd_loop_kernel<T><<<dim3(a.rows), dim3(1024), 0, st>>>(a);
@@ -424,13 +437,20 @@ void backward_t(const NormGradArgs& a, hipStream_t st) {
   const dim3 grid(blocks), block(s.tpr <= 64 ? 256 : s.tpr);
 #define CPD_NORM(TPR, CH)                                     \
   if (s.tpr == TPR && s.ch == CH) {                           \
-    norm_bwd_kernel<T, TPR, CH><<<grid, block, 0, st>>>(a);   \
+    norm_bwd_kernel<T, TPR, CH, DS><<<grid, block, 0, st>>>(a); \
     return;                                                   \
   }
-  CPD_NORM(16, 1) CPD_NORM(16, 2) CPD_NORM(16, 4)
-  CPD_NORM(64, 2) CPD_NORM(64, 4)
-  CPD_NORM(256, 2) CPD_NORM(256, 4)
-  CPD_NORM(1024, 2) CPD_NORM(1024, 4)
+  if constexpr (sizeof(T) == 4) {
+    CPD_NORM(16, 1) CPD_NORM(16, 2) CPD_NORM(16, 4)
+    CPD_NORM(64, 2) CPD_NORM(64, 4)
+    CPD_NORM(256, 2) CPD_NORM(256, 4)
+    CPD_NORM(1024, 2) CPD_NORM(1024, 4)
+  } else {
+    CPD_NORM(16, 1) CPD_NORM(16, 2)
+    CPD_NORM(64, 1) CPD_NORM(64, 2)
+    CPD_NORM(256, 1) CPD_NORM(256, 2)
+    CPD_NORM(1024, 1) CPD_NORM(1024, 2)
+  }
 #undef CPD_NORM
 }
 
@@ -447,7 +467,7 @@ void norm_forward(const NormArgs& a, hipStream_t st) {
 }
 
 int norm_grad_blocks(long rows, int cols, Dt dt) {
-  const Shape s = shape_for(cols, dt);
+  const Shape s = backward_shape(cols, dt);
   if (s.tpr == 0) return (int)(rows < 64 ? rows : 64);
   const long per = s.tpr <= 64 ? 256 / s.tpr : 1;
   const long groups = (rows + per - 1) / per;
@@ -457,12 +477,18 @@ int norm_grad_blocks(long rows, int cols, Dt dt) {
 
 void norm_backward(const NormGradArgs& a, hipStream_t st) {
   if (a.rows == 0) return;
+  auto start = [&](auto zero) {
+    if (a.ds)
+      backward_t<decltype(zero), true>(a, st);
+    else
+      backward_t<decltype(zero), false>(a, st);
+  };
   if (a.dt == Dt::f32)
-    backward_t<float>(a, st);
+    start(0.f);
   else if (a.dt == Dt::bf16)
-    backward_t<bf16_t>(a, st);
+    start((bf16_t)0.f);
   else
-    backward_t<f16_t>(a, st);
+    start((f16_t)0.f);
   if (a.partial)
     norm_bwd_join_kernel<<<dim3((2L * a.cols + 31) / 32), dim3(1024), 0, st>>>(
         a.partial, norm_grad_blocks(a.rows, a.cols, a.dt), a.cols, a.dweight,
