@@ -11,34 +11,39 @@
 //
 // Everything is bound by memory: each pass reads its inputs once and writes
 // its outputs once.  A row stays in the registers of the threads that share
-// it (16 threads, a wave, a block of 256 or of 1024), so the variance is
+// it (16 threads, a wave, a block of 256 to 1024), so the variance is
 // taken around the mean without a second read.  All sums are 32-bit floats.
 //
 // With bf16 rows of 4096 and the residual, 8192 of them take 60 us forward and
-// 62 + 5 backward (268 MB each: 4.4 TB/s, where a copy of 1 GiB runs at 4.9);
-// 20011 float rows of 257 take 12 and 20 + 4 (3.4 TB/s).
+// 61 + 4 backward (268 MB each: 4.5 and 4.1 TB/s, where a copy of 1 GiB runs at
+// 4.9); 20011 float rows of 257 take 12 and 18 + 4 (3.3 and 2.8 TB/s).
 #include "fused_ops.h"
 
 namespace cpd {
 namespace {
 
-// Threads that share a row, and 16-byte chunks each of them holds.  A row of
-// more than 4096 chunks goes to the looping kernels below.
+// Threads that share a row, and 16-byte chunks each of them holds.  Longer rows
+// go to the looping kernels below.  (us for 2^25 values:)
+//  - Forward up to four chunks: bf16 rows of 8192 took 34, with two 47, floats of
+//    4096 43 and 58; 512 threads where 256 are too few: floats of 5120 56, with
+//    1024 threads 81, bf16 of 12288 42 and 49.
+//  - Backward four of floats (1024: 81, with two 106), but two in 16 bits, whose
+//    sums of columns take twice the registers (512: 46, with four 84; 8192: 50 and
+//    107).
 struct Shape {
   int tpr, ch;
 };
 
-Shape shape_for(int cols, Dt dt, int most) {
+Shape shape_for(int cols, Dt dt, int most, bool half) {
   const int vec = 16 / dt_size(dt);
   const int n = (cols + vec - 1) / vec;
-  const int tprs[4] = {16, 64, 256, 1024};
-  for (int t : tprs)
-    if (n <= t * most) return {t, n <= t ? 1 : n <= 2 * t ? 2 : 4};
+  for (int t : {16, 64, 256, 512, 1024})
+    if (n <= t * most && (t != 512 || half)) return {t, n <= t ? 1 : n <= 2 * t ? 2 : 4};
   return {0, 0};
 }
-Shape forward_shape(int cols, Dt dt) { return shape_for(cols, dt, 4); }
+Shape forward_shape(int cols, Dt dt) { return shape_for(cols, dt, 4, true); }
 Shape backward_shape(int cols, Dt dt) {
-  return shape_for(cols, dt, dt == Dt::f32 ? 4 : 2);
+  return shape_for(cols, dt, dt == Dt::f32 ? 4 : 2, false);
 }
 
 template <typename T, int TPR, int CH>
@@ -184,7 +189,8 @@ __global__ __launch_bounds__(1024) void norm_fwd_loop_kernel(NormArgs a) {
 // dweight and dbias in registers (a thread has the same columns in every
 // row), so the data is read once for all three gradients; the next row is
 // ordered before this one is worked on, since the two sums over the row leave
-// memory idle otherwise.  The blocks' shares go to `partial` and are added in a
+// memory idle otherwise (not in blocks of 1024, which have registers for one:
+// 16384 bf16 took 221 us for 2^25 values with two, 83 with one).  The blocks' shares go to `partial` and are added in a
 // fixed order: no atomics.
 template <typename T, int TPR, int CH, bool DS>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_bwd_kernel(
@@ -419,7 +425,7 @@ void forward_t(const NormArgs& a, hipStream_t st) {
   CPD_NORM(16, 1) CPD_NORM(16, 2) CPD_NORM(16, 4)
   CPD_NORM(64, 2) CPD_NORM(64, 4)
   CPD_NORM(256, 2) CPD_NORM(256, 4)
-  CPD_NORM(1024, 2) CPD_NORM(1024, 4)
+  CPD_NORM(512, 4) CPD_NORM(1024, 4)
 #undef CPD_NORM
 }
 
@@ -471,6 +477,8 @@ int norm_grad_blocks(long rows, int cols, Dt dt) {
   if (s.tpr == 0) return (int)(rows < 64 ? rows : 64);
   const long per = s.tpr <= 64 ? 256 / s.tpr : 1;
   const long groups = (rows + per - 1) / per;
+  // (us for 2^25 values of bf16, rows of 256, 2048 and 16384: 42, 50 and 66; with
+  // half the blocks 54, 74 and 73; with twice as many 60, 55 and 94)
   const long most = s.tpr == 1024 ? 256 : 512;
   return (int)(groups < most ? groups : most);
 }
