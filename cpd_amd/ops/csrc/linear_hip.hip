@@ -23,8 +23,9 @@ namespace {
 // The activations and their slopes.  What is stored in 16 bits takes the
 // machine's exp2 and reciprocal (1 ulp each) and, for the normal distribution's
 // cdf, the polynomial of Abramowitz and Stegun 7.1.26 (1.5e-7 off at most, a
-// two-thousandth of fp16's half step at 1), whose exponential is the density's
-// too: erff alone is some 40 instructions, which bound the gradient's pass.
+// two-thousandth of fp16's half step at 1; of gelu's own value in the far tail
+// 7e-4 at -4.2, 3e-3 at -5.7 and 7e-3 at -7.1, where that is 5e-12), whose
+// exponential is the density's too: erff alone is some 40 instructions, which bound the gradient's pass.
 template <bool EXACT>
 __device__ __forceinline__ float exp_of(float x) {
   return EXACT ? expf(x) : __builtin_amdgcn_exp2f(x * 1.4426950408889634f);
@@ -69,10 +70,13 @@ __device__ __forceinline__ float act_value(float z, Act act) {
   }
 }
 
-// (relu's is a choice, not a factor: an infinite gradient times zero is NaN)
+// (relu's is a choice, not a factor: an infinite gradient times zero is NaN.  An
+// argument that 16 bits do not hold is kept as an infinity, where the slopes have
+// their limits: 0 and 1.)
 template <typename T>
 __device__ __forceinline__ float act_slope(float z, Act act) {
   constexpr bool EXACT = __is_same(T, float);
+  if (!EXACT && fabsf(z) == INFINITY) return z > 0.f ? 1.f : 0.f;
   switch (act) {
     case Act::gelu: {
       float density;

@@ -1281,3 +1281,55 @@ def test_gpu_logprobs_top_many_rows():
         want = torch.sort(x[at].double(), dim=-1, descending=True,
                           stable=True)[1][:, :20]
         assert torch.equal(out.top_ids[at], want)
+
+
+@on_devices
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_linear_argument_out_of_range(device, act):
+    """An argument that fp16 does not hold: far below zero value and slope are
+    zero, not NaN."""
+    x = torch.full((3, 8), 100.0, dtype=torch.float16, device=device)
+    w = torch.full((5, 8), -100.0, dtype=torch.float16, device=device)
+    w[1] = 0.25
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    b = torch.zeros(5, dtype=torch.float16, device=device, requires_grad=True)
+    y = fused_linear(x, w, b, act)
+    assert torch.equal(y[:, [0, 2, 3, 4]], torch.zeros_like(y[:, :4]))
+    y.backward(torch.ones_like(y))
+    assert torch.equal(b.grad, torch.tensor([0, 3, 0, 0, 0.]).to(b))
+    assert torch.equal(x.grad, torch.full_like(x, 0.25))
+    assert torch.equal(w.grad[0], torch.zeros_like(w[0]))
+    assert torch.equal(w.grad[1], torch.full_like(w[1], 300.0))
+
+
+# the last length of each way of sharing a row, forward and backward, in 16 and
+# in 32 bits, and the next one
+@on_devices
+@on_types
+@pytest.mark.parametrize("cols", [
+    64, 65, 128, 129, 256, 257, 1024, 1025, 1028, 4096, 4100, 4104, 8192, 8200,
+    16392, 32768, 32776])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_lengths(device, dtype, cols, residual):
+    run_norm(device, dtype, 5, cols, residual)
+
+
+@pytest.mark.gpu
+def test_gpu_linear_far_offsets():
+    """Outputs and gradients whose offsets pass 2^31 elements."""
+    m, k, n = (1 << 19) + 5, 64, 4200
+    x = torch.randint(-2, 3, (m, k), device="cuda").bfloat16()
+    w = torch.randint(-2, 3, (n, k), device="cuda").bfloat16()
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    y = fused_linear(x, w, None, "relu")
+    dy = torch.zeros_like(y)
+    dy[-3:] = 1
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    z = x.detach()[-3:].double() @ w.detach().double().t()
+    assert torch.equal(y[-3:], z.clamp_min(0).bfloat16())
+    dz = (z > 0).double()
+    assert torch.equal(dx[-3:], (dz @ w.detach().double()).bfloat16())
+    assert not dx[:-3].any()
+    assert torch.equal(dw, (dz.t() @ x.detach()[-3:].double()).bfloat16())
