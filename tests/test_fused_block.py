@@ -1333,3 +1333,21 @@ def test_gpu_linear_far_offsets():
     assert torch.equal(dx[-3:], (dz @ w.detach().double()).bfloat16())
     assert not dx[:-3].any()
     assert torch.equal(dw, (dz.t() @ x.detach()[-3:].double()).bfloat16())
+
+
+@on_devices
+@pytest.mark.parametrize("m", [8, 200])
+@pytest.mark.parametrize("scale", [1e-30, 1e-34, 1e-37, 1e30])
+def test_linear_small_and_large_floats(device, m, scale):
+    """Beside the sum's rounding an input may lose two parts of less than
+    2^-126 each."""
+    g = rng(m, 31)
+    x = normal(g, m, 64, dtype=torch.float64, device="cpu",
+               scale=scale).float()
+    w = normal(g, 40, 64, dtype=torch.float32, device="cpu")
+    y = fused_linear(x.to(device), w.to(device))
+    x, w = x.double(), w.double()
+    want = x @ w.t()
+    size = x.abs() @ w.abs().t()
+    within(y, want, (64 + 64) * U * size + 2.0 ** -125 * w.abs().sum(-1)
+           + stored(want, torch.float32))
