@@ -91,6 +91,7 @@ struct GemmArgs {
   Operand a, b;
   int m, n, k;
   Dt dt;              // of A, B, y, z, residual
+  bool wide;          // A is float, whatever dt is
   void* y;            // [m, n], row stride y_ld: act(C + bias) + residual
   long y_ld;
   void* z;            // [m, n] contiguous: C + bias, or null
@@ -114,6 +115,9 @@ constexpr long kMostFeatures = 1L << 22;
 // bytes at a time; if not, pad_rows makes a copy that it takes.  Floats are
 // taken as they lie, and so is everything along with gemm_few_rows.
 bool gemm_takes(const Operand& o, long rows);
+// Whether dz is kept in floats behind an activation that makes new numbers of it:
+// products of m by n by k multiplications at most, whose time is the launch's.
+bool gemm_keeps_floats(long m, long n, long k, Dt dt, Act act);
 bool gemm_few_rows(long m, long n, long k, Dt dt);
 void pad_rows(const void* from, long ld, void* to, long to_ld, int rows,
               int cols, Dt dt, hipStream_t stream);
@@ -127,6 +131,7 @@ struct ActGradArgs {
   const void* z;      // [m, n], row stride z_ld; for relu the output may stand in
   long z_ld;
   void* dz;           // [m, n], row stride dz_ld, or null
+  bool wide;          // dz is float, whatever dt is
   long dz_ld;
   void* dbias;        // [n] or null
   Dt bias_dt;

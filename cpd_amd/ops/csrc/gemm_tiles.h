@@ -198,7 +198,11 @@ __device__ __forceinline__ s16x8 fragment(const char* half, int row, int kk,
 // against the float matrix instructions' 0.157; 0.20 are measured at 8192 x 2048
 // by 8192, where the library's float product has 0.15.
 //
-// What is not finite becomes (+-1, 0, x): the third part meets first parts
+// Where a 16-bit product gets one operand in floats (dz), both are cut into two
+// parts, which is exact for the 16-bit one and leaves 16 bits of the other, and
+// three products are kept.
+//
+// What is not finite becomes (+-1, 0, x): the last part meets first parts
 // only, which are zero for zeros alone, so inf times 0 is NaN, inf times
 // anything else inf, and no part of a finite number makes a NaN of it.
 // (Parts below the normal range, 2^-126, count as zero: floats below 1e-33 lose
@@ -211,18 +215,19 @@ __device__ __forceinline__ int swizzle_float(int r) { return r >> 1 & 3; }
 constexpr int kFloatK = 32;
 constexpr int kPlane = 8192;
 
-// One thread's share of 128 rows by 32 k: eight floats.
-template <bool ACROSS>
+// One thread's share of 128 rows by 32 k: eight floats (or what T has for them),
+// cut into P parts.
+template <typename T, int P, bool ACROSS>
 struct FloatStager {
-  const float* p;  // of this thread's eight, in the first tile
-  long step;       // floats from a tile to the next
+  const T* p;      // of this thread's eight, in the first tile
+  long step;       // elements from a tile to the next
   int at;          // along: its first k; across: its k
   int rows_left;   // across: rows from its first on
   u32 place;       // where its 16 bytes of a plane belong
 
   __device__ __forceinline__ void start(const Operand& o, int row0, int rows,
                                         int tid) {  // of 512
-    const float* base = static_cast<const float*>(o.p);
+    const T* base = static_cast<const T*>(o.p);
     if constexpr (!ACROSS) {
       const int r = tid >> 2, chunk = tid & 3;
       at = chunk * 8;
@@ -242,13 +247,13 @@ struct FloatStager {
 
   // `left`: k from this tile's first on
   __device__ __forceinline__ void load(int tile, int left, float (&v)[8]) const {
-    const float* q = p + tile * step;
+    const T* q = p + tile * step;
     const int n = ACROSS ? (at < left ? rows_left : 0) : left - at;
-    load_some<float, 8>(q, n, v);
+    load_some<T, 8>(q, n, v);
   }
 
   __device__ __forceinline__ void store(char* lds, const float (&v)[8]) const {
-    u32 part[3][4];
+    u32 part[P][4];
     u32 most = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i]) << 1);
@@ -266,7 +271,8 @@ struct FloatStager {
       // the upper halves of two, side by side
       part[0][i] = __builtin_amdgcn_perm(first[1], first[0], 0x07060302u);
       part[1][i] = __builtin_amdgcn_perm(second[1], second[0], 0x07060302u);
-      part[2][i] = __builtin_amdgcn_perm(third[1], third[0], 0x07060302u);
+      if (P > 2)
+        part[P - 1][i] = __builtin_amdgcn_perm(third[1], third[0], 0x07060302u);
     }
     if (most >= 0xFF000000u) {  // an infinity or NaN among the eight
 #pragma unroll
@@ -278,12 +284,12 @@ struct FloatStager {
         const u32 top = (u >> 16) | (u << 9 ? 0x40u : 0u);
         part[0][i / 2] = (part[0][i / 2] & keep) |
                          ((0x3F80u | (u >> 16 & 0x8000u)) << sh);
-        part[1][i / 2] = part[1][i / 2] & keep;
-        part[2][i / 2] = (part[2][i / 2] & keep) | (top << sh);
+        if (P > 2) part[1][i / 2] = part[1][i / 2] & keep;
+        part[P - 1][i / 2] = (part[P - 1][i / 2] & keep) | (top << sh);
       }
     }
 #pragma unroll
-    for (int q = 0; q < 3; ++q) {
+    for (int q = 0; q < P; ++q) {
       typedef u32 V __attribute__((ext_vector_type(4)));
       *reinterpret_cast<V*>(lds + q * kPlane + place) =
           V{part[q][0], part[q][1], part[q][2], part[q][3]};

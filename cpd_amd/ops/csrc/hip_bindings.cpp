@@ -338,10 +338,11 @@ struct Products {
   hipStream_t st;
   std::vector<Tensor> keep;
 
-  cpd::Operand operand(const Rows& r, bool across, bool padded, bool few,
+  // `any`: the kernel takes it as it lies
+  cpd::Operand operand(const Rows& r, bool across, bool padded, bool any,
                        const Tensor& like) {
     cpd::Operand o{r.p, r.ld, across, padded};
-    if (few || dt == Dt::f32 || r.rows == 0 ||
+    if (any || dt == Dt::f32 || r.rows == 0 ||
         cpd::gemm_takes(o, across ? r.cols : r.rows))
       return o;
     const int64_t ld = whole_lines(r.cols);
@@ -474,9 +475,11 @@ std::vector<Tensor> linear_bwd(const Tensor& dy, const Tensor& x,
   const bool fits =
       dt == Dt::f32 || ((!need_x || cpd::gemm_takes({g.p, g.ld, false, false}, m)) &&
                         (!need_w || cpd::gemm_takes({g.p, g.ld, true, false}, n)));
+  const bool wide = cpd::gemm_keeps_floats(m, n, k, dt, p.act);
   if ((need_x || need_w) && (p.act != cpd::Act::none || !fits)) {
     g.ld = whole_lines(n);
-    dz = at::empty({m, g.ld}, x.options());
+    dz = at::empty({m, g.ld}, wide ? x.options().dtype(at::kFloat) : x.options());
+    p.wide = wide;
     p.dz = dz.mutable_data_ptr();
     p.dz_ld = g.ld;
     g.p = p.dz;
@@ -496,18 +499,19 @@ std::vector<Tensor> linear_bwd(const Tensor& dy, const Tensor& x,
   const bool padded = p.dz != nullptr;
   cpd::GemmArgs q{}, v{};
   q.dt = q.bias_dt = v.dt = v.bias_dt = dt;
+  q.wide = v.wide = wide;
   q.n = v.n = (int)k;
   q.y_ld = v.y_ld = k;
   if (need_x) {
-    q.a = products.operand(g, false, padded, false, x);
-    q.b = products.operand(w, true, false, false, x);
+    q.a = products.operand(g, false, padded, wide, x);
+    q.b = products.operand(w, true, false, wide, x);
     q.m = (int)m;
     q.k = (int)n;
     q.y = dx.mutable_data_ptr();
   }
   if (need_w) {
-    v.a = products.operand(g, true, padded, false, x);
-    v.b = products.operand(r, true, false, false, x);
+    v.a = products.operand(g, true, padded, wide, x);
+    v.b = products.operand(r, true, false, wide, x);
     v.m = (int)n;
     v.k = (int)m;
     v.y = dw.mutable_data_ptr();

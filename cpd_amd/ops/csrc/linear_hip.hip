@@ -436,15 +436,17 @@ __device__ __forceinline__ void tile_128(const GemmArgs& g, int id, char* lds) {
                     slice);
 }
 
-// 128 by 128 results of floats (gemm_tiles.h), tiles of 32 k.  Waves 4-11 read
+// 128 by 128 results of floats, or of a float A and a B of T (gemm_tiles.h: P
+// parts of each), tiles of 32 k.  Waves 4-11 read
 // floats three tiles ahead, cut them into planes and write those to LDS; waves
 // 0-3, one on each SIMD beside two of the others, multiply 64 by 64 each.  So
 // the cutting goes on under the matrix instructions (1536 cycles a tile).  With
 // both done by all of eight waves in turn a tile took 1.6 us, with four waves
 // that cut 1.3 us, which was their time.
-template <bool AX, bool BX>
+template <typename T, bool AX, bool BX>
 __device__ __forceinline__ void tile_floats(const GemmArgs& g, int id,
                                             char* lds) {
+  constexpr int P = __is_same(T, float) ? 3 : 2;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tm = (g.m + 127) / 128, tn = (g.n + 127) / 128, slices = g.slices;
@@ -461,8 +463,8 @@ __device__ __forceinline__ void tile_floats(const GemmArgs& g, int id,
     block_barrier();
   };
   if (wave >= 4) {
-    FloatStager<AX> sa;
-    FloatStager<BX> sb;
+    FloatStager<float, P, AX> sa;
+    FloatStager<T, P, BX> sb;
     sa.start(g.a, m0, g.m, threadIdx.x - 256);
     sb.start(g.b, n0, g.n, threadIdx.x - 256);
     struct Raw {
@@ -476,9 +478,9 @@ __device__ __forceinline__ void tile_floats(const GemmArgs& g, int id,
     // writes tile t, orders tile t + 3 in its place
     auto step = [&](int t, Raw& r) {
       if (t >= to) return;
-      char* buf = lds + ((t - from) & 1) * (6 * kPlane);
+      char* buf = lds + ((t - from) & 1) * (2 * P * kPlane);
       sa.store(buf, r.a);
-      sb.store(buf + 3 * kPlane, r.b);
+      sb.store(buf + P * kPlane, r.b);
       load(t + 3, r);
       // tile t is there; and tile t - 1 has been read, whose place t + 1 takes
       meet();
@@ -498,18 +500,18 @@ __device__ __forceinline__ void tile_floats(const GemmArgs& g, int id,
   f32x4 acc[4][4] = {};
   for (int t = from; t < to; ++t) {
     meet();
-    const char* buf = lds + ((t - from) & 1) * (6 * kPlane);
-    s16x8 fa[3][4], fb[3][4];
+    const char* buf = lds + ((t - from) & 1) * (2 * P * kPlane);
+    s16x8 fa[P][4], fb[P][4];
 #pragma unroll
-    for (int q = 0; q < 3; ++q)
+    for (int q = 0; q < P; ++q)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         fa[q][i] = float_fragment<AX>(buf + q * kPlane, wm + i * 16, lane);
-        fb[q][i] = float_fragment<BX>(buf + (3 + q) * kPlane, wn + i * 16, lane);
+        fb[q][i] = float_fragment<BX>(buf + (P + q) * kPlane, wn + i * 16, lane);
       }
     // in the order in which the planes arrive
 #pragma unroll
-    for (int sum = 0; sum < 3; ++sum)
+    for (int sum = 0; sum < P; ++sum)
 #pragma unroll
       for (int q = 0; q <= sum; ++q)
 #pragma unroll
@@ -520,21 +522,27 @@ __device__ __forceinline__ void tile_floats(const GemmArgs& g, int id,
   }
   // The producers wrote their last tile before the last barrier; but the other
   // waves may still be reading it, so each wave leaves through the half of LDS
-  // that the last tile is not in, 12 KB a wave: 48 rows, then 16.
-  char* free = lds + ((to - from) & 1) * (6 * kPlane) + wave * 12288;
-  leave_block<float, 3>(g, free, acc, m0 + wm, n0 + wn, lane, slice);
-  leave_block<float, 1>(g, free, acc + 3, m0 + wm + 48, n0 + wn, lane, slice);
+  // that the last tile is not in, 4 P KB a wave: 48 rows, then 16, or 32 twice.
+  char* free = lds + ((to - from) & 1) * (2 * P * kPlane) + wave * (P * 4096);
+  leave_block<T, P>(g, free, acc, m0 + wm, n0 + wn, lane, slice);
+  leave_block<T, 4 - P>(g, free, acc + P, m0 + wm + P * 16, n0 + wn, lane, slice);
 }
 
-template <typename T>
-constexpr int kThreads = __is_same(T, float) ? 768 : 512;
-template <typename T>
-constexpr int kLds = __is_same(T, float) ? 12 * kPlane : 8 * kHalf;
+// What a launch's tiles are: 256 or 128 (of floats 128 by 32 k), or kWide, those
+// of a float A and a 16-bit B.
+constexpr int kWide = 1;
+
+template <typename T, int TILE>
+constexpr int kThreads = __is_same(T, float) || TILE == kWide ? 768 : 512;
+template <typename T, int TILE>
+constexpr int kLds = __is_same(T, float) ? 12 * kPlane
+                     : TILE == kWide     ? 8 * kPlane
+                                         : 8 * kHalf;
 
 template <typename T, bool AX, bool BX, int TILE>
 __device__ __forceinline__ void tile_any(const GemmArgs& g, int id, char* lds) {
-  if constexpr (__is_same(T, float))
-    tile_floats<AX, BX>(g, id, lds);
+  if constexpr (__is_same(T, float) || TILE == kWide)
+    tile_floats<T, AX, BX>(g, id, lds);
   else if constexpr (TILE == 256)
     tile_256<T, AX, BX>(g, id, lds);
   else
@@ -542,9 +550,9 @@ __device__ __forceinline__ void tile_any(const GemmArgs& g, int id, char* lds) {
 }
 
 template <typename T, bool AX, bool BX, int TILE>
-__global__ __launch_bounds__(kThreads<T>, kThreads<T> / 256) void gemm_kernel(
-    GemmArgs g) {
-  __shared__ __attribute__((aligned(1024))) char lds[kLds<T>];
+__global__ __launch_bounds__((kThreads<T, TILE>),
+                             (kThreads<T, TILE> / 256)) void gemm_kernel(GemmArgs g) {
+  __shared__ __attribute__((aligned(1024))) char lds[kLds<T, TILE>];
   tile_any<T, AX, BX, TILE>(g, blockIdx.x, lds);
 }
 
@@ -553,9 +561,10 @@ __global__ __launch_bounds__(kThreads<T>, kThreads<T> / 256) void gemm_kernel(
 // in two launches and takes 102, of 512 x 2048 by 1000 floats 56 and 46.  `first`
 // blocks are dx's, or dW's if those take longer.
 template <typename T, int DX, int DW>
-__global__ __launch_bounds__(kThreads<T>, kThreads<T> / 256) void gemm_two_kernel(
-    GemmArgs dx, GemmArgs dw, int first, bool dw_first) {
-  __shared__ __attribute__((aligned(1024))) char lds[kLds<T>];
+__global__ __launch_bounds__((kThreads<T, DX>), (kThreads<T, DX> / 256)) void
+gemm_two_kernel(GemmArgs dx, GemmArgs dw, int first, bool dw_first) {
+  static_assert(kThreads<T, DX> == kThreads<T, DW>, "one block, one size");
+  __shared__ __attribute__((aligned(1024))) char lds[kLds<T, DX>];
   const int id = blockIdx.x;
   const bool second = id >= first;
   if (second == dw_first)
@@ -732,7 +741,7 @@ struct Plan {
 };
 
 Plan plan_of(const GemmArgs& g, int tile, int slices) {
-  const bool floats = g.dt == Dt::f32;
+  const bool floats = g.dt == Dt::f32 || g.wide;
   const long tile_k = floats ? kFloatK : kTileK;
   const long tiles = (g.k + tile_k - 1) / tile_k;
   const long tm = (g.m + tile - 1) / tile, tn = (g.n + tile - 1) / tile;
@@ -745,8 +754,9 @@ Plan plan_of(const GemmArgs& g, int tile, int slices) {
 // Calls f with the ways there are; at least four tiles of k a slice.
 template <typename F>
 void each_plan(const GemmArgs& g, bool powers, F f) {
-  if (g.dt != Dt::f32) f(plan_of(g, 256, 1));
-  const long tiles = g.k / (g.dt == Dt::f32 ? kFloatK : kTileK);
+  const bool floats = g.dt == Dt::f32 || g.wide;
+  if (!floats) f(plan_of(g, 256, 1));
+  const long tiles = g.k / (floats ? kFloatK : kTileK);
   for (int s = 1; s <= 32 && (s == 1 || tiles / s >= 4); s = powers ? 2 * s : s + 1)
     f(plan_of(g, 128, s));
 }
@@ -794,8 +804,12 @@ void join_slices(const GemmArgs& g, hipStream_t st) {
 
 template <typename T, bool AX, bool BX>
 void gemm_tiles_t(const GemmArgs& g, hipStream_t st) {
-  const dim3 grid(blocks_of(g)), threads(kThreads<T>);
-  if (g.tile == 256) {
+  const dim3 grid(blocks_of(g)), threads(kThreads<T, 128>);
+  if (g.wide) {
+    if constexpr (!__is_same(T, float) && BX)
+      gemm_kernel<T, AX, BX, kWide>
+          <<<grid, dim3(kThreads<T, kWide>), 0, st>>>(g);
+  } else if (g.tile == 256) {
     if constexpr (!__is_same(T, float))
       gemm_kernel<T, AX, BX, 256><<<grid, threads, 0, st>>>(g);
   } else if (g.tile == 128) {
@@ -832,12 +846,15 @@ void gemm_two_tiles(const GemmArgs& dx, const GemmArgs& dw, hipStream_t st) {
   const bool dw_first = plan_of(dw, dw.tile, dw.slices).block >
                         plan_of(dx, dx.tile, dx.slices).block;
   const unsigned nx = blocks_of(dx), nw = blocks_of(dw);
-  const dim3 grid(nx + nw), threads(kThreads<T>);
+  const dim3 grid(nx + nw), threads(kThreads<T, 128>);
   const int first = (int)(dw_first ? nw : nx);
   if constexpr (__is_same(T, float)) {
     gemm_two_kernel<T, 128, 128><<<grid, threads, 0, st>>>(dx, dw, first, dw_first);
   } else {
-    if (dx.tile == 256 && dw.tile == 256)
+    if (dx.wide)
+      gemm_two_kernel<T, kWide, kWide>
+          <<<grid, dim3(kThreads<T, kWide>), 0, st>>>(dx, dw, first, dw_first);
+    else if (dx.tile == 256 && dw.tile == 256)
       gemm_two_kernel<T, 256, 256><<<grid, threads, 0, st>>>(dx, dw, first, dw_first);
     else if (dx.tile == 256)
       gemm_two_kernel<T, 256, 128><<<grid, threads, 0, st>>>(dx, dw, first, dw_first);
@@ -883,7 +900,10 @@ __global__ __launch_bounds__(256) void act_grad_kernel(ActGradArgs a,
           g[i] = a.act == Act::relu ? (z[i] > 0.f ? g[i] : 0.f)
                                     : g[i] * act_slope<T>(z[i], a.act);
       }
-      if (a.dz)
+      if (a.dz && a.wide)
+        store_some<float, VEC>(static_cast<float*>(a.dz) + (long)row * a.dz_ld + col,
+                               left, g);
+      else if (a.dz)
         store_vec<T>(static_cast<T*>(a.dz) + (long)row * a.dz_ld + col, left, g);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sum[i] += g[i];
@@ -1001,6 +1021,11 @@ bool gemm_plan_two(GemmArgs& a, GemmArgs& b) {
 
 long gemm_work(const GemmArgs& g) {
   return g.slices > 1 ? (long)g.slices * g.m * g.n : 0;
+}
+
+bool gemm_keeps_floats(long m, long n, long k, Dt dt, Act act) {
+  return dt != Dt::f32 && (act == Act::gelu || act == Act::silu) &&
+         m * n * k <= 1L << 28;
 }
 
 bool gemm_takes(const Operand& o, long rows) {
