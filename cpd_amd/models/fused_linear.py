@@ -68,8 +68,9 @@ def fused_linear(x, weight, bias=None, activation=None, residual=None):
     float32.  ``activation`` is None, "relu", "gelu" (x times the normal
     distribution's cdf) or "silu".  Sums are 32-bit; the result is rounded
     once.  For the backward pass of gelu and silu their argument is kept in
-    ``x``'s type, and in 16 bits the gradient behind the activation is rounded
-    to that type too.  Of float32 inputs the GPU may leave out what lies below
+    ``x``'s type; where the products are large (over 2^28 multiplications, or
+    2^24 weights) and 16-bit, the gradient behind the activation is rounded to
+    that type too.  Of float32 inputs the GPU may leave out what lies below
     2^-125.
 
     Rows may be apart by any stride; the result is contiguous.  Raises

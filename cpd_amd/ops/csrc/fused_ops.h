@@ -116,7 +116,7 @@ constexpr long kMostFeatures = 1L << 22;
 // taken as they lie, and so is everything along with gemm_few_rows.
 bool gemm_takes(const Operand& o, long rows);
 // Whether dz is kept in floats behind an activation that makes new numbers of it:
-// products of m by n by k multiplications at most, whose time is the launch's.
+// where the products' time is the launch's.
 bool gemm_keeps_floats(long m, long n, long k, Dt dt, Act act);
 bool gemm_few_rows(long m, long n, long k, Dt dt);
 void pad_rows(const void* from, long ld, void* to, long to_ld, int rows,

@@ -729,8 +729,8 @@ namespace {
 
 // How a product is cut up, and the time that it takes.  The tile kernels have
 // one block a CU, so time goes by rounds of 256 blocks.  In units of a 128-tile's
-// 64 k (0.48 us): a 256-tile's take 2.4, 32 k of floats 2.3, what a block does
-// before and behind its loop 10 and 16, and the joining kernel 8 and 8 bytes for
+// 64 k (0.48 us): a 256-tile's take 2.4, 32 k of floats 2.3 (taken for a float A
+// beside 16 bits too, which are below), what a block does before and behind its loop 10 and 16, and the joining kernel 8 and 8 bytes for
 // each partial sum at 4 TB/s.
 struct Plan {
   int tile;      // 256 or 128; 32 or 16 for gemm_rows_kernel
@@ -1023,9 +1023,15 @@ long gemm_work(const GemmArgs& g) {
   return g.slices > 1 ? (long)g.slices * g.m * g.n : 0;
 }
 
+// (dz rounded to 16 bits makes dx and dW 1.45 times as far from 64 bits as one
+// rounding of theirs does, kept in floats 1.05.  The kernels of a backward pass
+// in us, rounded and kept: 100 x 1000 by 1000 26 and 26, 128 x 1024 by 1024 20
+// and 25, 1 x 4096 by 4096 37 and 49, while a pass is 75 of the host's time;
+// beyond these sizes it costs more: 1 x 16384 by 4096 95 and 140, 1024 x 1024 by
+// 1024 26 and 45, 2048^3 58 and 163.)
 bool gemm_keeps_floats(long m, long n, long k, Dt dt, Act act) {
   return dt != Dt::f32 && (act == Act::gelu || act == Act::silu) &&
-         m * n * k <= 1L << 28;
+         m * n * k <= 1L << 28 && n * k <= 1L << 24;
 }
 
 bool gemm_takes(const Operand& o, long rows) {

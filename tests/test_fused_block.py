@@ -1351,3 +1351,59 @@ def test_linear_small_and_large_floats(device, m, scale):
     size = x.abs() @ w.abs().t()
     within(y, want, (64 + 64) * U * size + 2.0 ** -125 * w.abs().sum(-1)
            + stored(want, torch.float32))
+
+
+# Behind gelu and silu small products keep the gradient in floats: what dx and
+# dW are off by is their own rounding and what z's makes of the slope.
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("m,k,n", [(1, 24, 4480), (12, 896, 54), (70, 130, 61),
+                                   (300, 520, 264), (2, 5, 3), (515, 33, 700)])
+def test_gpu_linear_gradients_rounded_once(dtype, act, m, k, n):
+    g = rng(m, k, n, 9)
+    x, dy = (normal(g, m, c, dtype=dtype, device="cuda") for c in (k, n))
+    w = normal(g, n, k, dtype=dtype, device="cuda", scale=k ** -0.5)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    dx, dw = torch.autograd.grad(fused_linear(x, w, None, act), [x, w], dy)
+    x64, w64, dy64 = (v.detach().cpu().double() for v in (x, w, dy))
+    z = x64 @ w64.t()
+    _, slope, bend = act_oracle(z, act)
+    dz = dy64 * slope
+    # a float cut to two parts keeps 16 bits: 2^-15 of it are lost at most, and
+    # the product of two second parts, 2^-16, is left out
+    cut = 2.0 ** -14
+    err_z = (k + 64) * U * (x64.abs() @ w64.abs().t())
+    err = dy64.abs() * (bend * (err_z + stored(z, dtype)) + 32 * U * (
+        1 + z.abs())) + cut * dz.abs()
+    for got, want, tol in (
+            (dx, dz @ w64, err @ w64.abs() + (n + 64) * U * (
+                dz.abs() @ w64.abs())),
+            (dw, dz.t() @ x64, err.t() @ x64.abs() + (m + 64) * U * (
+                dz.abs().t() @ x64.abs()))):
+        within(got, want, tol + stored(want, dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m", [40, 4100])
+def test_gpu_linear_gradients_not_finite(dtype, m):
+    """Infinities and a NaN reach their own rows and columns and no others,
+    on both sides of the size from which the gradient is rounded."""
+    k, n = 72, 1024
+    x = torch.ones(m, k, dtype=dtype, device="cuda")
+    w = torch.full((n, k), 2.0 ** -7, dtype=dtype, device="cuda")
+    dy = torch.ones(m, n, dtype=dtype, device="cuda")
+    x[2, 4] = w[5, 7] = math.inf   # z infinite there: a slope of one
+    dy[3, 9] = math.nan
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    dx, dw = torch.autograd.grad(fused_linear(x, w, None, "silu"), [x, w], dy)
+    for got, row, col in ((dx, 3, 7), (dw, 9, 4)):
+        kinds = torch.zeros(got.shape, device="cuda")
+        kinds[:, col] = 1
+        kinds[row] = 2
+        assert torch.equal(got == math.inf, kinds == 1)
+        assert torch.equal(got.isnan(), kinds == 2)
+        assert torch.equal(got.isfinite(), kinds == 0)
