@@ -729,8 +729,9 @@ namespace {
 
 // How a product is cut up, and the time that it takes.  The tile kernels have
 // one block a CU, so time goes by rounds of 256 blocks.  In units of a 128-tile's
-// 64 k (0.48 us): a 256-tile's take 2.4, 32 k of floats 2.3 (taken for a float A
-// beside 16 bits too, which are below), what a block does before and behind its loop 10 and 16, and the joining kernel 8 and 8 bytes for
+// 64 k (0.48 us): a 256-tile's take 2.4, 32 k of floats 2.3 (also taken for a
+// float A beside 16 bits, which has half the instructions), what a block does
+// before and behind its loop 10 and 16, and the joining kernel 8 and 8 bytes for
 // each partial sum at 4 TB/s.
 struct Plan {
   int tile;      // 256 or 128; 32 or 16 for gemm_rows_kernel
