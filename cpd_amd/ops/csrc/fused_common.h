@@ -149,6 +149,16 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
+// The largest of a wave's values, NaN passed over.
+__device__ __forceinline__ float group_max(float v) {
+  v = fmaxf(v, rotate16<8>(v));
+  v = fmaxf(v, rotate16<4>(v));
+  v = fmaxf(v, rotate16<2>(v));
+  v = fmaxf(v, rotate16<1>(v));
+  return fmaxf(fmaxf(lane_value(v, 0), lane_value(v, 16)),
+               fmaxf(lane_value(v, 32), lane_value(v, 48)));
+}
+
 // Sums of two values over the TPR threads that share a row: within a wave by
 // lanes, over waves through `smem` (4 TPR/64 floats).  `turn` alternates 0/1
 // from call to call, so that one barrier a call is enough.

@@ -1407,3 +1407,12 @@ def test_gpu_linear_gradients_not_finite(dtype, m):
         assert torch.equal(got == math.inf, kinds == 1)
         assert torch.equal(got.isnan(), kinds == 2)
         assert torch.equal(got.isfinite(), kinds == 0)
+
+
+# a row cut into the most parts, whose lists are joined 64 keys at a time or one
+# by one
+@on_devices
+@pytest.mark.parametrize("top_k", [1, 8, 15, 16, 64])
+def test_logprobs_top_of_many_parts(device, top_k):
+    x, t = make_logits(rng(top_k), torch.bfloat16, device, 3, 140001)
+    run_logprobs(device, x, t, top_k)
