@@ -341,10 +341,17 @@ __device__ __forceinline__ void tile_128(const GemmArgs& g, int id, char* lds) {
   const int left = slice == slices - 1 ? g.k % kTileK : 0;
 
   f32x4 acc[4][4] = {};
+  // With one row of tiles, blocks are bound by reading B, and with its rows a
+  // multiple of 4 KB apart all that is read at a time, 128 bytes a row, lies on a
+  // few memory channels: each block begins elsewhere in its k.
+  const bool apart = tm == 1 && !BX && (g.b.ld * 2) % 4096 == 0 && to > from;
+  const int turn = apart ? (bn * 5 + slice * 3) % (to - from) : 0;
   auto copy = [&](int t) {
     const u32 at = lds0 + ((t - from) & 3) * (2 * kHalf);
-    ca.half(t, 0, at);
-    cb.half(t, 0, at + kHalf);
+    int k = t + turn;
+    k = k < to ? k : k - (to - from);
+    ca.half(k, 0, at);
+    cb.half(k, 0, at + kHalf);
   };
   struct Fragments {
     s16x8 a[4], b[4];

@@ -1416,3 +1416,30 @@ def test_gpu_linear_gradients_not_finite(dtype, m):
 def test_logprobs_top_of_many_parts(device, top_k):
     x, t = make_logits(rng(top_k), torch.bfloat16, device, 3, 140001)
     run_logprobs(device, x, t, top_k)
+
+
+# Few rows and large weights, whose rows lie a power of two apart or not: blocks
+# then begin at different places of k, and wrap round
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n", [
+    (33, 64, 131100), (48, 130, 66000), (64, 384, 22000), (40, 448, 19000),
+    (64, 2104, 4100), (48, 8200, 1100), (34, 40000, 257), (48, 16384, 520),
+    (128, 4096, 300), (100, 2048, 4200), (65, 10240, 1000), (1, 16384, 40),
+    (7, 4096, 1000), (20, 8192, 260), (32, 2048, 2050)])
+def test_gpu_linear_large_weights(dtype, m, k, n):
+    """Whole numbers: equal to the formula in 64 bits, rounded once."""
+    g = torch.Generator(device="cuda").manual_seed(m + k + n)
+    draw = lambda *s: torch.randint(  # noqa: E731
+        -2, 3, s, generator=g, device="cuda").to(dtype)
+    x, w, b, res = draw(m, k), draw(n, k), draw(n) + 0.5, draw(m, n)
+    want = (x.double() @ w.double().t() + b.double()).clamp_min(0)
+    assert torch.equal(fused_linear(x, w, b, "relu", res),
+                       (want + res.double()).to(dtype))
+    # a misaligned start, and a k that ends inside a tile of wider rows
+    wide = torch.cat([x, x], 1)[:, 3:k + 3]
+    want = wide.double() @ w.double().t()
+    assert torch.equal(fused_linear(wide, w), want.to(dtype))
+    x, w = x[:, :k - 21], w[:, :k - 21]
+    assert torch.equal(fused_linear(x, w),
+                       (x.double() @ w.double().t()).to(dtype))
