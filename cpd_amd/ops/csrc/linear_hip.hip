@@ -343,7 +343,8 @@ __device__ __forceinline__ void tile_128(const GemmArgs& g, int id, char* lds) {
   f32x4 acc[4][4] = {};
   // With one row of tiles, blocks are bound by reading B, and with its rows a
   // multiple of 4 KB apart all that is read at a time, 128 bytes a row, lies on a
-  // few memory channels: each block begins elsewhere in its k.
+  // few memory channels: each block begins elsewhere in its k (48 rows with
+  // 134 MB, k 16384: 35 us, 41 without).
   const bool apart = tm == 1 && !BX && (g.b.ld * 2) % 4096 == 0 && to > from;
   const int turn = apart ? (bn * 5 + slice * 3) % (to - from) : 0;
   auto copy = [&](int t) {
@@ -587,10 +588,12 @@ gemm_two_kernel(GemmArgs dx, GemmArgs dw, int first, bool dw_first) {
 // for alignment.  Where there are few blocks and much k, `slices` of them share
 // a row's k as above.
 //
-// A is read once for every 16 W rows of B, which limits how many rows pay: with
-// 134 MB of 16-bit B, 8, 16, 32 and 48 rows took 34, 39, 50 and 66 us for W = 1
-// and 34, 37, 40 and 50 for W = 2 against 40 of gemm_128_kernel; with 34 MB 11,
-// 12, 16 and 21 against 17; with 8 MB 6, 7, 7 and 9 against 14.
+// A is read once for every 16 W rows of B, which limits how many rows pay.  With
+// 134 MB of 16-bit B (k 4096, k 16384, k 5000) 1 row takes 26, 29 and 34 us, 16
+// take 28, 32 and 43, 32 take 36, 39 and 55, and by tiles of 128 16 take 34, 34
+// and 41, 32 take 31, 33 and 42; with 34 MB 16 take 10, 32 take 14 and by tiles 15;
+// with 8 MB 32 and 48 took 7 and 9, by tiles 14.  With 134 MB of floats 32 take 48,
+// by tiles 54.
 template <typename T, int F, int W>
 __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g) {
   constexpr int VEC = 16 / sizeof(T);    // a lane's elements of a load
@@ -606,6 +609,10 @@ __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g) {
   const int per = (units + g.slices - 1) / g.slices;
   const int from = slice * per, to = min(from + per, units);
   const int k0 = (lane >> 4) * 2 * VEC;
+  // (as in tile_128: with all blocks from their first k on 1 row and k 4096 took 31
+  // us instead of 26, with steps of a whole kilobyte between them 30)
+  const bool apart = (g.b.ld * (long)sizeof(T)) % 4096 == 0 && to > from;
+  const int turn = apart ? (int)(blockIdx.x * 5) % (to - from) : 0;
   // (rows behind the last one repeat it: their results are not stored)
   const T *a[F], *b[W];
 #pragma unroll
@@ -638,8 +645,9 @@ __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g) {
   auto load = [&](int u, Lines& l) {
 #pragma unroll
     for (int q = 0; q < BATCH; ++q) {
-      const int k = (u + q * 8) * UNIT;
       const bool in = u + q * 8 < to;
+      const int at = u + q * 8 + turn;
+      const int k = (at < to ? at : at - (to - from)) * UNIT;
 #pragma unroll
       for (int w = 0; w < W; ++w) fetch(b[w], k, in, l.b[q][w]);
 #pragma unroll
@@ -729,7 +737,9 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs g) {
 
 // Whether gemm_rows_kernel takes a product of operands along (its figures).
 bool gemm_few_rows(long m, long n, long k, Dt dt) {
-  return m <= 32 || (m <= 64 && n * k * dt_size(dt) <= (16L << 20));
+  const long bytes = n * k * dt_size(dt);
+  return m <= 16 || (m <= 32 && (dt == Dt::f32 || bytes <= (48L << 20))) ||
+         (m <= 64 && bytes <= (16L << 20));
 }
 
 namespace {
@@ -831,9 +841,12 @@ void gemm_tiles_t(const GemmArgs& g, hipStream_t st) {
     const integral_constant<int, 1> one;
     const integral_constant<int, 2> two;
     const integral_constant<int, 4> four;
-    if (g.tile == 32)
-      g.m <= 16 ? start(one, two) : start(two, two);
-    else
+    if (g.tile == 32) {
+      if constexpr (__is_same(T, float))
+        g.m <= 16 ? start(one, two) : start(two, two);
+      else
+        start(one, two);  // (more rows go to tiles: gemm_few_rows)
+    } else
       g.m <= 16 ? start(one, one) : g.m <= 32 ? start(two, one) : start(four, one);
   }
   join_slices<T>(g, st);
@@ -987,7 +1000,8 @@ void gemm_plan(GemmArgs& g) {
   g.slices = 1;
   if (g.m < 1 || g.n < 1) return;  // nothing will be launched
   if (!g.a.across && !g.b.across && gemm_few_rows(g.m, g.n, g.k, g.dt)) {
-    // 16 rows of B a block, or 32 where A would be read too often
+    // 16 rows of B a block, or 32 where A would be read too often (1 row with 134
+    // MB and k 5000: 34 us, with 16 of B 43; with 34 MB 16 are faster)
     const long bytes = (long)g.n * g.k * dt_size(g.dt);
     g.tile = g.m <= 32 && bytes > (48L << 20) ? 32 : 16;
     const long blocks = (g.n + g.tile - 1) / g.tile;

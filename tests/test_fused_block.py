@@ -1443,3 +1443,18 @@ def test_gpu_linear_large_weights(dtype, m, k, n):
     x, w = x[:, :k - 21], w[:, :k - 21]
     assert torch.equal(fused_linear(x, w),
                        (x.double() @ w.double().t()).to(dtype))
+
+
+# both sides of the sizes up to which few rows go straight from memory
+@pytest.mark.gpu
+@on_types
+@pytest.mark.parametrize("m", [16, 17, 32, 33, 64, 65])
+@pytest.mark.parametrize("k,n", [(2048, 4090), (2048, 4102), (4096, 6100),
+                                 (4096, 6200)])
+def test_gpu_linear_few_rows(dtype, m, k, n):
+    g = torch.Generator(device="cuda").manual_seed(m + k + n)
+    draw = lambda *s: torch.randint(  # noqa: E731
+        -2, 3, s, generator=g, device="cuda").to(dtype)
+    x, w, b = draw(m, k), draw(n, k), draw(n)
+    assert torch.equal(fused_linear(x, w, b), (
+        x.double() @ w.double().t() + b.double()).to(dtype))
