@@ -25,7 +25,8 @@ namespace {
 // cdf, the polynomial of Abramowitz and Stegun 7.1.26 (1.5e-7 off at most, a
 // two-thousandth of fp16's half step at 1; of gelu's own value in the far tail
 // 7e-4 at -4.2, 3e-3 at -5.7 and 7e-3 at -7.1, where that is 5e-12), whose
-// exponential is the density's too: erff alone is some 40 instructions, which bound the gradient's pass.
+// exponential is the density's too: erff alone is some 40 instructions, which
+// bound the gradient's pass.
 template <bool EXACT>
 __device__ __forceinline__ float exp_of(float x) {
   return EXACT ? expf(x) : __builtin_amdgcn_exp2f(x * 1.4426950408889634f);
@@ -319,7 +320,7 @@ __device__ __forceinline__ void tile_256(const GemmArgs& g, int id, char* lds) {
 // tile took 0.74 us) and copies have three steps to land.  One barrier a
 // step: a wave that has passed it has its copies of tile t + 1 and knows that
 // all have read tile t, whose place tile t + 4 takes.  The tiles of k may be
-// shared out over `slices` blocks, whose sums then go to `part` as they are.
+// shared out over `slices` blocks, whose sums then go to the workspace as they are.
 template <typename T, bool AX, bool BX>
 __device__ __forceinline__ void tile_128(const GemmArgs& g, int id, char* lds) {
   const int lane = threadIdx.x & 63;

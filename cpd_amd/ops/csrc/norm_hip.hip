@@ -190,8 +190,8 @@ __global__ __launch_bounds__(1024) void norm_fwd_loop_kernel(NormArgs a) {
 // row), so the data is read once for all three gradients; the next row is
 // ordered before this one is worked on, since the two sums over the row leave
 // memory idle otherwise (not in blocks of 1024, which have registers for one:
-// 16384 bf16 took 221 us for 2^25 values with two, 83 with one).  The blocks' shares go to `partial` and are added in a
-// fixed order: no atomics.
+// 16384 bf16 took 221 us for 2^25 values with two, 83 with one).  The blocks'
+// shares go to `partial` and are added in a fixed order: no atomics.
 template <typename T, int TPR, int CH, bool DS>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_bwd_kernel(
     NormGradArgs a) {
