@@ -919,7 +919,8 @@ __global__ __launch_bounds__(256) void act_grad_kernel(ActGradArgs a,
                     0.f, z);
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
-          g[i] = a.act == Act::relu ? (z[i] > 0.f ? g[i] : 0.f)
+          // (a NaN argument is not below zero: its gradient goes through, as it did)
+          g[i] = a.act == Act::relu ? (z[i] <= 0.f ? 0.f : g[i])
                                     : g[i] * act_slope<T>(z[i], a.act);
       }
       if (a.dz && a.wide)

@@ -1458,3 +1458,27 @@ def test_gpu_linear_few_rows(dtype, m, k, n):
     x, w, b = draw(m, k), draw(n, k), draw(n)
     assert torch.equal(fused_linear(x, w, b), (
         x.double() @ w.double().t() + b.double()).to(dtype))
+
+
+@on_devices
+@on_types
+@pytest.mark.parametrize("residual", [False, True])
+def test_linear_relu_of_nan(device, dtype, residual):
+    """relu leaves NaN as it is, and its gradient too: only what is zero or
+    below takes it away."""
+    x = torch.tensor([[math.nan, 1], [2, 1], [-3, 1], [-1, 1], [-math.inf, 1]],
+                     dtype=dtype, device=device, requires_grad=True)
+    w = torch.ones(3, 2, dtype=dtype, device=device, requires_grad=True)
+    b = torch.zeros(3, dtype=dtype, device=device, requires_grad=True)
+    res = torch.ones(5, 3, dtype=dtype, device=device) if residual else None
+    y = fused_linear(x, w, b, "relu", res)
+    more = 1.0 if residual else 0.0
+    assert y[0].isnan().all()
+    assert torch.equal(y[1:, 0].cpu(),
+                       torch.tensor([3.0, 0, 0, 0], dtype=dtype) + more)
+    y.backward(torch.ones_like(y))
+    live = torch.tensor([1.0, 1, 0, 0, 0], dtype=dtype)
+    assert torch.equal(x.grad.cpu(), 3 * live[:, None].expand(5, 2))
+    assert torch.equal(b.grad.cpu(), torch.full((3,), 2.0, dtype=dtype))
+    assert w.grad[:, 0].isnan().all()
+    assert torch.equal(w.grad[:, 1].cpu(), torch.full((3,), 2.0, dtype=dtype))
