@@ -25,7 +25,7 @@ void norm_forward(const NormArgs& a, hipStream_t stream);
 
 struct NormGradArgs {
   const void* s;          // what was normalised [rows, cols], row stride s_ld
-  const void* dy;         // or null: zero
+  const void* dy;         // [rows, cols], row stride dy_ld
   const void* ds;         // added to the result, or null
   const void* weight;     // or null
   const float* stats;     // [rows, 2]

@@ -159,7 +159,7 @@ std::vector<Tensor> norm_fwd(const Tensor& x, const OptTensor& weight,
 }
 
 // dx, dweight, dbias
-std::vector<Tensor> norm_bwd(const Tensor& s, const OptTensor& dy,
+std::vector<Tensor> norm_bwd(const Tensor& s, const Tensor& dy,
                              const OptTensor& ds, const OptTensor& weight,
                              const Tensor& stats, bool need_w, bool need_b,
                              at::ScalarType bias_type) {
@@ -173,13 +173,11 @@ std::vector<Tensor> norm_bwd(const Tensor& s, const OptTensor& dy,
                         stats.scalar_type() == at::kFloat,
                     "stats are not this input's");
   check_on(stats, s, "stats");
-  Rows g, h;
-  if (dy.has_value() && dy->defined()) {
-    check_like(*dy, s, "the output's gradient");
-    g = rows_of(*dy);
-    a.dy = g.p;
-    a.dy_ld = g.ld;
-  }
+  check_like(dy, s, "the output's gradient");
+  const Rows g = rows_of(dy);
+  a.dy = g.p;
+  a.dy_ld = g.ld;
+  Rows h;
   if (ds.has_value() && ds->defined()) {
     check_like(*ds, s, "the sum's gradient");
     h = rows_of(*ds);
@@ -586,12 +584,20 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     check_once("layer norm");
     const Tensor ds = g.size() > 1 ? g[1] : Tensor();
     if (!g[0].defined() && !ds.defined()) return variable_list(5);
+    const bool x = needs(ctx, "x"), w = needs(ctx, "weight"),
+               b = needs(ctx, "bias"), res = needs(ctx, "residual");
+    const auto type = ctx->saved_data["type"].toScalarType();
+    if (!g[0].defined()) {
+      // Only the sum was used: its gradient is x's and the residual's as it is,
+      // also in rows whose norm is not finite.
+      const auto none = [&](bool need) {
+        return need ? at::zeros({ds.size(-1)}, ds.options().dtype(type)) : Tensor();
+      };
+      return {x ? ds : Tensor(), none(w), none(b), Tensor(), res ? ds : Tensor()};
+    }
     const auto saved = ctx->get_saved_variables();
-    auto d = norm_bwd(saved[0], some(g[0]), some(ds), some(saved[1]), saved[2],
-                      needs(ctx, "weight"), needs(ctx, "bias"),
-                      ctx->saved_data["type"].toScalarType());
-    return {needs(ctx, "x") ? d[0] : Tensor(), d[1], d[2], Tensor(),
-            needs(ctx, "residual") ? d[0] : Tensor()};
+    auto d = norm_bwd(saved[0], g[0], some(ds), some(saved[1]), saved[2], w, b, type);
+    return {x ? d[0] : Tensor(), d[1], d[2], Tensor(), res ? d[0] : Tensor()};
   }
 };
 

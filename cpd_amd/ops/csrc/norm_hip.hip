@@ -212,8 +212,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_bwd_kernel(
     for (int c = 0; c < CH; ++c) {
       const int at = (c * TPR + lane) * VEC, left = a.cols - at;
       r.s[c] = load_raw<T>(static_cast<const T*>(a.s) + row * a.s_ld + at, left);
-      r.dy[c] = load_raw<T>(static_cast<const T*>(a.dy) + row * a.dy_ld + at,
-                            a.dy ? left : 0);
+      r.dy[c] = load_raw<T>(static_cast<const T*>(a.dy) + row * a.dy_ld + at, left);
       if constexpr (DS)
         r.ds[c] = load_raw<T>(static_cast<const T*>(a.ds) + row * a.ds_ld + at, left);
     }
@@ -322,9 +321,9 @@ __global__ __launch_bounds__(1024) void norm_bwd_loop_kernel(NormGradArgs a) {
   for (int pass = 0; pass < 2; ++pass) {
     for (long at = threadIdx.x * VEC; at < a.cols; at += 1024 * VEC) {
       const int left = (int)(a.cols - at);
-      float h[VEC], g[VEC] = {}, w[VEC];
+      float h[VEC], g[VEC], w[VEC];
       load_vec<T>(s + at, left, mean, h);
-      if (a.dy) load_vec<T>(dy + at, left, 0.f, g);
+      load_vec<T>(dy + at, left, 0.f, g);
       if (a.weight) load_learned<VEC>(a.weight, a.wdt, at, left, w);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
@@ -362,8 +361,7 @@ __global__ __launch_bounds__(256) void norm_bwd_cols_kernel(NormGradArgs a) {
   if (col >= a.cols) return;
   float dw = 0.f, db = 0.f;
   for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
-    const float g =
-        a.dy ? (float)static_cast<const T*>(a.dy)[row * a.dy_ld + col] : 0.f;
+    const float g = (float)static_cast<const T*>(a.dy)[row * a.dy_ld + col];
     const float s = (float)static_cast<const T*>(a.s)[row * a.s_ld + col];
     dw += g * ((s - a.stats[row * 2]) * a.stats[row * 2 + 1]);
     db += g;

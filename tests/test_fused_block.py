@@ -1482,3 +1482,27 @@ def test_linear_relu_of_nan(device, dtype, residual):
     assert torch.equal(b.grad.cpu(), torch.full((3,), 2.0, dtype=dtype))
     assert w.grad[:, 0].isnan().all()
     assert torch.equal(w.grad[:, 1].cpu(), torch.full((3,), 2.0, dtype=dtype))
+
+
+@on_devices
+@on_types
+@pytest.mark.parametrize("eps", [1e-5, 0.0])
+@pytest.mark.parametrize("cols", [24, 40000])
+def test_norm_only_the_sum_used(device, dtype, eps, cols):
+    """Where only s = x + residual goes on, its gradient is both inputs', also
+    in rows that have no norm: an infinity, a NaN, no spread and no eps."""
+    g = rng(cols, 77)
+    x = normal(g, 4, cols, dtype=dtype, device=device)
+    x[0, 1], x[1, 2] = math.inf, math.nan
+    x[2] = 3.0
+    res = torch.zeros_like(x).requires_grad_(True)
+    x.requires_grad_(True)
+    w, b = (torch.ones(cols, dtype=dtype, device=device, requires_grad=True)
+            for _ in range(2))
+    ds = normal(g, 4, cols, dtype=dtype, device=device)
+    _, s = fused_layer_norm(x, w, b, eps, res)
+    dx, dres, dw, db = torch.autograd.grad(s, [x, res, w, b], ds,
+                                           allow_unused=True)
+    assert torch.equal(dx, ds) and torch.equal(dres, ds)
+    for v in (dw, db):
+        assert v is None or torch.equal(v, torch.zeros_like(w))
