@@ -205,8 +205,11 @@ __device__ __forceinline__ s16x8 fragment(const char* half, int row, int kk,
 // What is not finite becomes (+-1, 0, x): the last part meets first parts
 // only, which are zero for zeros alone, so inf times 0 is NaN, inf times
 // anything else inf, and no part of a finite number makes a NaN of it.
-// (Parts below the normal range, 2^-126, count as zero: floats below 1e-33 lose
-// their last bits, up to 2^-125 in all.)
+//
+// bf16 ends at 2^-133: what a float has below that is cut off (of floats under
+// 2^-109, 1.5e-33; at 1e-36 that is 1e-4 of the value), and a float that is all
+// below it counts as 2^-133, so that its first part is not zero.  So each operand
+// is off by 2^-133 at most.
 //
 // Tiles are of 32 k and three planes of 8 KB: along, row r of 64 bytes with
 // its chunk c at place c ^ r/2 % 4; across, as above.
@@ -254,9 +257,10 @@ struct FloatStager {
 
   __device__ __forceinline__ void store(char* lds, const float (&v)[8]) const {
     u32 part[P][4];
-    u32 most = 0;
+    // NaN, infinities and what is below the normal range: one instruction each
+    bool odd = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i]) << 1);
+    for (int i = 0; i < 8; ++i) odd |= __builtin_amdgcn_classf(v[i], 0x297);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       u32 first[2], second[2], third[2];
@@ -274,18 +278,21 @@ struct FloatStager {
       if (P > 2)
         part[P - 1][i] = __builtin_amdgcn_perm(third[1], third[0], 0x07060302u);
     }
-    if (most >= 0xFF000000u) {  // an infinity or NaN among the eight
+    if (odd) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const u32 u = __float_as_uint(v[i]);
-        if ((u << 1) < 0xFF000000u) continue;
         const u32 sh = (i & 1) * 16, keep = i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-        // (a NaN whose bits are all in the lower half must stay one)
-        const u32 top = (u >> 16) | (u << 9 ? 0x40u : 0u);
-        part[0][i / 2] = (part[0][i / 2] & keep) |
-                         ((0x3F80u | (u >> 16 & 0x8000u)) << sh);
-        if (P > 2) part[1][i / 2] = part[1][i / 2] & keep;
-        part[P - 1][i / 2] = (part[P - 1][i / 2] & keep) | (top << sh);
+        if ((u << 1) >= 0xFF000000u) {
+          // (a NaN whose bits are all in the lower half must stay one)
+          const u32 top = (u >> 16) | (u << 9 ? 0x40u : 0u);
+          part[0][i / 2] = (part[0][i / 2] & keep) |
+                           ((0x3F80u | (u >> 16 & 0x8000u)) << sh);
+          if (P > 2) part[1][i / 2] = part[1][i / 2] & keep;
+          part[P - 1][i / 2] = (part[P - 1][i / 2] & keep) | (top << sh);
+        } else if ((u << 1) - 1 < 0x1FFFFu) {
+          part[0][i / 2] |= 1u << sh;  // 2^-133; its parts are zeros, with its sign
+        }
       }
     }
 #pragma unroll

@@ -1506,3 +1506,45 @@ def test_norm_only_the_sum_used(device, dtype, eps, cols):
     assert torch.equal(dx, ds) and torch.equal(dres, ds)
     for v in (dw, db):
         assert v is None or torch.equal(v, torch.zeros_like(w))
+
+
+@on_devices
+@pytest.mark.parametrize("m", [8, 70, 200])
+def test_linear_infinity_times_a_tiny_float(device, m):
+    """An infinity times any float but zero is an infinity, however small that
+    is, forward and in both gradients."""
+    tiny = [2.0 ** -149, 2.0 ** -140, -2.0 ** -134, 2.0 ** -133, 2.0 ** -126,
+            -1e-37, 1e-30, 1.0, 0.0]
+    n = len(tiny)
+    small = torch.tensor(tiny, device=device)
+    # (the row that holds the infinity, in each operand)
+    x = torch.zeros(m, 8, device=device)
+    w = torch.zeros(n, 8, device=device)
+    x[1, 3] = math.inf
+    w[:, 3] = small
+    want = torch.where(small == 0, math.nan, small * math.inf)
+    same = lambda a, b: torch.equal(  # noqa: E731
+        a.nan_to_num(5, 6, 7), b.nan_to_num(5, 6, 7))
+    assert same(fused_linear(x, w)[1], want)
+    x[1, 3], w[:, 3] = 0, 0
+    x[:n, 3] = small[:m]
+    w[2, 3] = -math.inf
+    got = fused_linear(x, w)[:, 2]
+    assert same(got[:n], -want[:m]) and got[n:].isnan().all()
+    # dx = dy W, dW = dy^T x
+    for big, little in (("dy", "w"), ("w", "dy"), ("dy", "x"), ("x", "dy")):
+        v = {"x": torch.zeros(m, 8, device=device),
+             "w": torch.zeros(n, 8, device=device),
+             "dy": torch.zeros(m, n, device=device)}
+        into = "x" if "w" in (big, little) else "w"
+        if into == "x":   # summed over n
+            (v["dy"][1, :1] if big == "dy" else v["w"][:1, 2]).fill_(math.inf)
+            (v["dy"][1, :1] if little == "dy" else v["w"][:1, 2]).fill_(
+                tiny[0])
+        else:             # summed over m
+            (v["dy"][:1, 1] if big == "dy" else v["x"][:1, 2]).fill_(math.inf)
+            (v["dy"][:1, 1] if little == "dy" else v["x"][:1, 2]).fill_(
+                tiny[0])
+        leaf = v[into].requires_grad_(True)
+        a, = torch.autograd.grad(fused_linear(v["x"], v["w"]), leaf, v["dy"])
+        assert a[1, 2] == math.inf
