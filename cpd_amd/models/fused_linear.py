@@ -67,11 +67,13 @@ def fused_linear(x, weight, bias=None, activation=None, residual=None):
     type (float32, bfloat16 or float16); ``bias`` [N] is of that type or
     float32.  ``activation`` is None, "relu", "gelu" (x times the normal
     distribution's cdf) or "silu".  Sums are 32-bit; the result is rounded
-    once.  For the backward pass of gelu and silu their argument is kept in
-    ``x``'s type; where the products are large (over 2^28 multiplications, or
-    2^24 weights) and 16-bit, the gradient behind the activation is rounded to
-    that type too.  Of float32 inputs the GPU may leave out what lies below
-    2^-125.
+    once.  For the backward pass an activation's argument is kept in ``x``'s
+    type; where the products behind gelu and silu are large (over 2^28
+    multiplications, or 2^24 weights) and 16-bit, the gradient behind the
+    activation is rounded to that type too.  Of float32 operands (the inputs
+    and, backward, the incoming gradient) the GPU may leave out what lies below
+    2^-133: that of forward depends on the number of rows and the weight's
+    size, that of both gradients does not.
 
     Rows may be apart by any stride; the result is contiguous.  Raises
     TypeError and ValueError for types and shapes that do not fit.

@@ -1548,3 +1548,35 @@ def test_linear_infinity_times_a_tiny_float(device, m):
         leaf = v[into].requires_grad_(True)
         a, = torch.autograd.grad(fused_linear(v["x"], v["w"]), leaf, v["dy"])
         assert a[1, 2] == math.inf
+
+
+@on_devices
+@pytest.mark.parametrize("m", [1, 8, 70, 200])
+@pytest.mark.parametrize("scale", [1e-30, 1e-34, 1e-36, 1e-37, 1e-40, 1e30])
+def test_linear_small_and_large_gradients(device, m, scale):
+    """Forward and both gradients with one operand of this size: beside the
+    sum's rounding each operand may be off by 2^-133, where bf16 ends."""
+    g = rng(m, 33)
+    k, n = 64, 40
+    tiny = 2.0 ** -133
+    draw = lambda *s, scale=1.0: normal(  # noqa: E731
+        g, *s, dtype=torch.float64, device="cpu", scale=scale).float()
+
+    def bound(a, b, want):  # of a @ b.t()
+        terms = a.shape[1]
+        return (terms + 64) * U * (a.abs() @ b.abs().t()) + tiny * (
+            a.abs().sum(-1)[:, None] + b.abs().sum(-1)) \
+            + terms * TINY[torch.float32] + stored(want, torch.float32)
+
+    def check(got, a, b, what):
+        a, b = a.double(), b.double()
+        want = a @ b.t()
+        within(got, want, bound(a, b, want), what)
+
+    x, w = draw(m, k, scale=scale), draw(n, k)
+    check(fused_linear(x.to(device), w.to(device)), x, w, "y")
+    x, dy = draw(m, k), draw(m, n, scale=scale)
+    leaves = [v.to(device).requires_grad_(True) for v in (x, w)]
+    dx, dw = torch.autograd.grad(fused_linear(*leaves), leaves, dy.to(device))
+    check(dx, dy, w.t(), "dx")
+    check(dw, dy.t(), x.t(), "dw")
