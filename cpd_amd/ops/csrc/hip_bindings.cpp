@@ -524,6 +524,39 @@ std::vector<Tensor> linear_bwd(const Tensor& dy, const Tensor& x,
   return {dx, dw, db};
 }
 
+// How the products of m rows, n features out and k in are cut up (without an
+// activation): tile and slices of forward, of dx and of dW, and whether a call
+// for both gradients takes one launch.  Which kernels run is not seen in the
+// results, and tests have to reach every one.
+std::vector<int64_t> linear_plan(int64_t m, int64_t n, int64_t k,
+                                 at::ScalarType type, bool need_x, bool need_w) {
+  check_sizes(m, n, k);
+  const Dt dt = type == at::kFloat      ? Dt::f32
+                : type == at::kBFloat16 ? Dt::bf16
+                                        : Dt::f16;
+  auto product = [&](int64_t rows, int64_t cols, int64_t sum, bool ax, bool bx) {
+    cpd::GemmArgs g{};
+    g.dt = dt;
+    g.m = (int)rows;
+    g.n = (int)cols;
+    g.k = (int)sum;
+    g.a.across = ax;
+    g.b.across = bx;
+    return g;
+  };
+  auto y = product(m, n, k, false, false), dx = product(m, k, n, false, true),
+       dw = product(n, k, m, true, true);
+  cpd::gemm_plan(y);
+  bool together = false;
+  if (need_x && need_w) {
+    together = cpd::gemm_plan_two(dx, dw);
+  } else {
+    cpd::gemm_plan(dx);
+    cpd::gemm_plan(dw);
+  }
+  return {y.tile, y.slices, dx.tile, dx.slices, dw.tile, dw.slices, together};
+}
+
 // ---------------------------------------------------------------------------
 // The operators with their gradients.  The graph's nodes are C++: a backward
 // pass through Python's own function class costs about 50 us of waiting for
@@ -686,6 +719,8 @@ std::vector<Tensor> token_logprobs(const Tensor& x, const Tensor& targets,
 void cpd_register_fused(pybind11::module_& m) {
   m.def("layer_norm", &layer_norm, "layer norm (+residual): [y] or [y, s]");
   m.def("linear", &linear, "act(x W^T + bias) + residual");
+  m.def("linear_plan", &linear_plan,
+        "[tile, slices] of y, dx and dW, and whether the last two share a launch");
   m.def("token_logprobs", &token_logprobs,
         "[logprobs, entropy] or [logprobs, entropy, top_ids, top_logprobs]");
 }

@@ -1580,3 +1580,44 @@ def test_linear_small_and_large_gradients(device, m, scale):
     dx, dw = torch.autograd.grad(fused_linear(*leaves), leaves, dy.to(device))
     check(dx, dy, w.t(), "dx")
     check(dw, dy.t(), x.t(), "dw")
+
+
+# The largest tiles in the gradients: both in launches of their own and in one,
+# and sums of one, two and three whole tiles of 64 (over n for dx, over m for dW)
+# with and without a rest.  The plan is asserted, so that a size which no longer
+# reaches its kernel is seen: (tile of dx, of dW, one launch).
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n,plan", [
+    (4096, 4096, 4096, (256, 256, False)), (4000, 3999, 3900, (256, 256, False)),
+    (1030, 5000, 1100, (256, 256, True)), (2048, 4096, 2048, (256, 256, True)),
+    (3900, 4090, 64, (256, 128, True)), (4096, 4096, 72, (256, 128, True)),
+    (3900, 4090, 128, (256, 128, True)), (4096, 4096, 133, (256, 128, True)),
+    (3900, 4090, 192, (256, 128, True)), (4096, 4090, 200, (256, 128, True)),
+    (64, 3900, 4090, (128, 256, True)), (72, 4096, 4096, (128, 256, True)),
+    (128, 3900, 4090, (128, 256, True)), (133, 4096, 4096, (128, 256, True)),
+    (192, 3900, 4090, (128, 256, True)), (200, 4096, 4090, (128, 256, True))])
+def test_gpu_linear_largest_tiles_in_gradients(dtype, m, k, n, plan):
+    """Whole numbers, so that every sum is exact: equal to the formula in 64
+    bits, rounded once; for both gradients, each alone, and again."""
+    from cpd_amd import ops
+    plan_of = ops.hip_ext().linear_plan
+    p = plan_of(m, n, k, dtype, True, True)
+    assert (p[2], p[4], bool(p[6])) == plan
+    # alone, a gradient with the largest tiles has them too (but where those
+    # paid for filling the CUs with the other one's)
+    alone = (plan_of(m, n, k, dtype, True, False)[2],
+             plan_of(m, n, k, dtype, False, True)[4])
+    if plan != (256, 256, True):
+        assert all(a == 256 for a, b in zip(alone, plan) if b == 256)
+    g = torch.Generator(device="cuda").manual_seed(m + k + n)
+    draw = lambda *s: torch.randint(  # noqa: E731
+        -2, 3, s, generator=g, device="cuda").to(dtype)
+    x, w, dy = draw(m, k), draw(n, k), draw(m, n)
+    want = ((dy.double() @ w.double()).to(dtype),
+            (dy.double().t().contiguous() @ x.double()).to(dtype))
+    for need in ((True, True), (True, False), (False, True), (True, True)):
+        a, b = (v.detach().requires_grad_(r) for v, r in zip((x, w), need))
+        fused_linear(a, b).backward(dy)
+        for v, r, c in zip((a, b), need, want):
+            assert torch.equal(v.grad, c) if r else v.grad is None
