@@ -1621,3 +1621,65 @@ def test_gpu_linear_largest_tiles_in_gradients(dtype, m, k, n, plan):
         fused_linear(a, b).backward(dy)
         for v, r, c in zip((a, b), need, want):
             assert torch.equal(v.grad, c) if r else v.grad is None
+
+
+def slope_case(dtype, m, k, n):
+    """Inputs of whole numbers and a power of two, so that the activation's
+    argument is exact before it is stored: z is about 1.5 in size."""
+    g = rng(m, k, n, 13)
+    draw = lambda *s: torch.randint(-7, 8, s, generator=g).double()  # noqa: E731
+    x = draw(m, k)
+    w = draw(n, k) * 2.0 ** -round(math.log2(18.7 * k ** 0.5 / 1.5))
+    dy = normal(g, m, n, dtype=dtype, device="cpu")
+    assert torch.equal(x.to(dtype).double(), x)
+    assert torch.equal(w.to(dtype).double(), w)
+    return x, w, dy.double()
+
+
+def times_one_rounding(got, want, dtype):
+    """The error's root mean square, in that of a single rounding."""
+    rms = lambda v: v.square().mean().sqrt()  # noqa: E731
+    return (rms(got.double() - want) / rms(want.to(dtype).double() - want)).item()
+
+
+# dx and dW of 500 numbers or more each, up to 2^28 multiplications: sums over
+# few and many rows and features
+ROUNDED_ONCE = [(1, 1000, 700), (12, 896, 54), (70, 130, 61), (300, 520, 264),
+                (515, 33, 700), (9, 64, 4480), (2000, 24, 40)]
+on_rounded_once = pytest.mark.parametrize("m,k,n", ROUNDED_ONCE)
+on_curved = pytest.mark.parametrize("act", ["gelu", "silu"])
+on_16_bits = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+
+
+# What dz in two bf16 parts adds (2^-15 of each term, of which n add up by their
+# squares: at most an eighth of fp16's rounding of a sum) is under 1 % of the
+# root mean square; dz rounded to the type makes it 1.41.  Halfway is 1.2.
+@on_16_bits
+@on_curved
+@on_rounded_once
+def test_rounding_twice_is_told_from_once(dtype, act, m, k, n):
+    """The measure of the next test on the formula in 64 bits: what it says of
+    a gradient whose dz was rounded, and of one whose dz was not."""
+    x, w, dy = slope_case(dtype, m, k, n)
+    dz = dy * act_oracle((x @ w.t()).to(dtype).double(), act)[1]
+    for a, b in ((dz, w.t()), (dz.t(), x.t())):
+        want = a @ b.t()
+        twice = (a.to(dtype).double() @ b.t()).to(dtype)
+        assert times_one_rounding(want.to(dtype), want, dtype) == 1
+        assert times_one_rounding(twice, want, dtype) > 1.3
+
+
+@pytest.mark.gpu
+@on_16_bits
+@on_curved
+@on_rounded_once
+def test_gpu_linear_gradients_off_by_one_rounding(dtype, act, m, k, n):
+    """Behind gelu and silu, the slope taken at the argument as it is stored:
+    dx and dW are each as near 64 bits as one rounding allows."""
+    x, w, dy = slope_case(dtype, m, k, n)
+    dz = dy * act_oracle((x @ w.t()).to(dtype).double(), act)[1]
+    a, b = (v.to(dtype).cuda().requires_grad_(True) for v in (x, w))
+    dx, dw = torch.autograd.grad(fused_linear(a, b, None, act), [a, b],
+                                 dy.to(dtype).cuda())
+    assert times_one_rounding(dx.cpu(), dz @ w, dtype) < 1.2
+    assert times_one_rounding(dw.cpu(), dz.t() @ x, dtype) < 1.2
