@@ -86,9 +86,18 @@ def _deps_of(obj):
     return [n for n in names if n.startswith(CSRC)]
 
 
-def _object_stale(obj, src):
+def _made_by(obj):
+    """The command that ``obj`` was finished by, or None."""
+    try:
+        with open(obj[:-2] + ".cmd") as f:
+            return f.read()
+    except OSError:
+        return None
+
+
+def _object_stale(obj, src, cmd):
     deps = _deps_of(obj)
-    if deps is None or not os.path.exists(obj):
+    if deps is None or not os.path.exists(obj) or _made_by(obj) != cmd:
         return True
     t = os.path.getmtime(obj)
     return any(not os.path.exists(s) or os.path.getmtime(s) > t
@@ -145,16 +154,24 @@ def build_hip(force=False, verbose=True):
     )
     os.makedirs(OBJ, exist_ok=True)
     objs = [os.path.join(OBJ, os.path.basename(s) + ".o") for s in srcs]
-    todo = [(s, o) for s, o in zip(srcs, objs)
-            if force or _object_stale(o, s)]
+    # An object is taken again only if this very command (its architecture and
+    # flags) made it, and came to its end.
+    jobs = [(s, o, compile_flags + ["-MMD", "-MF", o[:-2] + ".d", "-c", s,
+                                    "-o", o]) for s, o in zip(srcs, objs)]
+    todo = [j for j in jobs
+            if force or _object_stale(j[1], j[0], " ".join(j[2]))]
 
     def compile_one(job):
-        src, obj = job
-        _run(compile_flags + ["-MMD", "-MF", obj[:-2] + ".d", "-c", src,
-                              "-o", obj], verbose)
+        _, obj, cmd = job
+        said = obj[:-2] + ".cmd"
+        if os.path.exists(said):
+            os.remove(said)
+        _run(cmd, verbose)
+        with open(said, "w") as f:
+            f.write(" ".join(cmd))
 
-    jobs = min(int(os.environ.get("MAX_JOBS", "8")), len(todo) or 1)
-    with ThreadPoolExecutor(max_workers=jobs) as pool:
+    workers = min(int(os.environ.get("MAX_JOBS", "8")), len(todo) or 1)
+    with ThreadPoolExecutor(max_workers=workers) as pool:
         list(pool.map(compile_one, todo))
     _run(["hipcc", f"--offload-arch={GFX_ARCH}", "-shared", "-fPIC",
           "-fno-gpu-rdc"] + objs + _link_flags(libs, hip=True)
