@@ -170,7 +170,7 @@ def build_hip(force=False, verbose=True):
         with open(said, "w") as f:
             f.write(" ".join(cmd))
 
-    workers = min(int(os.environ.get("MAX_JOBS", "8")), len(todo) or 1)
+    workers = max(1, min(int(os.environ.get("MAX_JOBS", "8")), len(todo)))
     with ThreadPoolExecutor(max_workers=workers) as pool:
         list(pool.map(compile_one, todo))
     _run(["hipcc", f"--offload-arch={GFX_ARCH}", "-shared", "-fPIC",

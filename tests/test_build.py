@@ -83,3 +83,9 @@ def test_a_killed_compiler_is_run_again(tree):
     tree.breaks = None
     tree.build()
     assert "a.hip" in tree.compiled
+
+
+def test_no_workers_asked_for(tree, monkeypatch):
+    monkeypatch.setenv("MAX_JOBS", "0")
+    tree.build()
+    assert len(tree.compiled) == 3
