@@ -34,9 +34,26 @@ Dt dtype_of(const Tensor& t, const char* name) {
   }
 }
 
+// The memory that a kernel reads or writes.  Tensors without any (of a wrapper
+// class, of a mode that only follows shapes, zeros known without being stored)
+// have address 0, which a kernel would go to.
+void check_memory(const void* p, const Tensor& t, const char* name) {
+  TORCH_CHECK_TYPE(p || t.numel() == 0, name, " has no memory of its own");
+}
+void check_memory(const Tensor& t, const char* name) {
+  check_memory(t.const_data_ptr(), t, name);
+}
+template <typename T = void>
+T* made(const Tensor& t) {
+  void* p = t.mutable_data_ptr();
+  check_memory(p, t, "a tensor made for the result");
+  return static_cast<T*>(p);
+}
+
 void check_on(const Tensor& t, const Tensor& x, const char* name) {
   TORCH_CHECK_VALUE(t.device() == x.device(), name, " is on ", t.device(),
                     ", the input on ", x.device());
+  check_memory(t, name);
 }
 
 void check_like(const Tensor& t, const Tensor& x, const char* name) {
@@ -92,6 +109,7 @@ Rows rows_of(const Tensor& t) {
   }
   r.ld = ld;
   r.p = r.keep.const_data_ptr();
+  check_memory(r.p, r.keep, "a tensor");
   return r;
 }
 
@@ -106,6 +124,7 @@ void check_launch(const char* what) {
 
 void check_input(const Tensor& x, const char* name) {
   TORCH_CHECK_VALUE(x.is_cuda(), name, " must be on the GPU");
+  check_memory(x, name);
 }
 
 // ---------------------------------------------------------------------------
@@ -136,7 +155,7 @@ std::vector<Tensor> norm_fwd(const Tensor& x, const OptTensor& weight,
     s = at::empty(x.sizes(), x.options());
     a.res = q.p;
     a.res_ld = q.ld;
-    a.s = s.mutable_data_ptr();
+    a.s = made(s);
   }
   TORCH_CHECK_VALUE(r.rows < (1L << 31), "layer norm takes less than 2^31 rows");
   TORCH_CHECK_VALUE(r.cols <= 16384 || r.rows < (1L << 22),
@@ -148,8 +167,8 @@ std::vector<Tensor> norm_fwd(const Tensor& x, const OptTensor& weight,
   a.weight = w ? w->const_data_ptr() : nullptr;
   a.bias = b ? b->const_data_ptr() : nullptr;
   a.wdt = w ? dtype_of(*w, "weight") : b ? dtype_of(*b, "bias") : a.dt;
-  a.y = y.mutable_data_ptr();
-  a.stats = stats.data_ptr<float>();
+  a.y = made(y);
+  a.stats = made<float>(stats);
   a.rows = r.rows;
   a.cols = (int)r.cols;
   a.eps = (float)eps;
@@ -195,15 +214,15 @@ std::vector<Tensor> norm_bwd(const Tensor& s, const Tensor& dy,
     partial = at::empty(
         {cpd::norm_grad_blocks(r.rows, (int)r.cols, a.dt), 2, r.cols},
         s.options().dtype(at::kFloat));
-    a.partial = partial.data_ptr<float>();
+    a.partial = made<float>(partial);
   }
   a.s = r.p;
   a.s_ld = r.ld;
   a.weight = w ? w->const_data_ptr() : nullptr;
   a.stats = stats.data_ptr<float>();
-  a.dx = dx.mutable_data_ptr();
-  a.dweight = need_w ? dw.mutable_data_ptr() : nullptr;
-  a.dbias = need_b ? db.mutable_data_ptr() : nullptr;
+  a.dx = made(dx);
+  a.dweight = need_w ? made(dw) : nullptr;
+  a.dbias = need_b ? made(db) : nullptr;
   a.rows = r.rows;
   a.cols = (int)r.cols;
   a.wdt = wtype == at::kFloat      ? Dt::f32
@@ -252,12 +271,12 @@ std::vector<Tensor> logprob_fwd(const Tensor& x, const Tensor& targets,
   a.x = r.p;
   a.ld = r.ld;
   a.targets = t.data_ptr<int64_t>();
-  a.logprobs = lp.data_ptr<float>();
-  a.entropy = ent.data_ptr<float>();
-  a.stats = stats.data_ptr<float>();
-  a.top_ids = top ? ids.mutable_data_ptr<int64_t>() : nullptr;
-  a.top_logprobs = top ? tops.data_ptr<float>() : nullptr;
-  a.work = bytes ? work.mutable_data_ptr() : nullptr;
+  a.logprobs = made<float>(lp);
+  a.entropy = made<float>(ent);
+  a.stats = made<float>(stats);
+  a.top_ids = top ? made<int64_t>(ids) : nullptr;
+  a.top_logprobs = top ? made<float>(tops) : nullptr;
+  a.work = bytes ? made(work) : nullptr;
   a.rows = r.rows;
   a.vocab = (int)r.cols;
   a.top = (int)top;
@@ -282,10 +301,12 @@ Tensor logprob_bwd(const Tensor& x, const Tensor& targets, const Tensor& stats,
   Tensor g, h;
   if (glp.has_value() && glp->defined()) g = glp->to(at::kFloat).contiguous();
   if (gent.has_value() && gent->defined()) h = gent->to(at::kFloat).contiguous();
-  for (const Tensor* v : {&g, &h})
+  for (const Tensor* v : {&g, &h}) {
+    if (v->defined()) check_memory(*v, "a gradient");
     TORCH_CHECK_VALUE(!v->defined() || (v->device() == x.device() &&
                                         v->numel() == r.rows),
                       "a gradient does not fit the logits");
+  }
   Tensor dx = at::empty(x.sizes(), x.options());
   a.x = r.p;
   a.ld = r.ld;
@@ -294,7 +315,7 @@ Tensor logprob_bwd(const Tensor& x, const Tensor& targets, const Tensor& stats,
   a.entropy = e.data_ptr<float>();
   a.glogprobs = g.defined() ? g.data_ptr<float>() : nullptr;
   a.gentropy = h.defined() ? h.data_ptr<float>() : nullptr;
-  a.dx = dx.mutable_data_ptr();
+  a.dx = made(dx);
   a.rows = r.rows;
   a.vocab = (int)r.cols;
   a.ignore = ignore;
@@ -345,7 +366,7 @@ struct Products {
       return o;
     const int64_t ld = whole_lines(r.cols);
     keep.push_back(at::empty({r.rows, ld}, like.options()));
-    cpd::pad_rows(r.p, r.ld, keep.back().mutable_data_ptr(), ld, (int)r.rows,
+    cpd::pad_rows(r.p, r.ld, made(keep.back()), ld, (int)r.rows,
                   (int)r.cols, dt, st);
     return {keep.back().const_data_ptr(), ld, across, true};
   }
@@ -355,7 +376,7 @@ struct Products {
     const long floats = cpd::gemm_work(g);
     if (!floats) return;
     keep.push_back(at::empty({floats}, like.options().dtype(at::kFloat)));
-    g.work = keep.back().data_ptr<float>();
+    g.work = made<float>(keep.back());
   }
 
   void run(cpd::GemmArgs& g, const Tensor& like) {
@@ -408,7 +429,7 @@ std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& weight,
   }
   if (want_z) {
     z = at::empty(shape, x.options());
-    g.z = z.mutable_data_ptr();
+    g.z = made(z);
   }
   Products products{g.dt, stream_of(x), {}};
   const bool few = cpd::gemm_few_rows(r.rows, w.rows, r.cols, g.dt);
@@ -417,7 +438,7 @@ std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& weight,
   g.m = (int)r.rows;
   g.n = (int)weight.size(0);
   g.k = (int)r.cols;
-  g.y = y.mutable_data_ptr();
+  g.y = made(y);
   g.y_ld = g.n;
   g.bias = b ? b->const_data_ptr() : nullptr;
   g.bias_dt = b ? dtype_of(*b, "bias") : g.dt;
@@ -478,17 +499,17 @@ std::vector<Tensor> linear_bwd(const Tensor& dy, const Tensor& x,
     g.ld = whole_lines(n);
     dz = at::empty({m, g.ld}, wide ? x.options().dtype(at::kFloat) : x.options());
     p.wide = wide;
-    p.dz = dz.mutable_data_ptr();
+    p.dz = made(dz);
     p.dz_ld = g.ld;
     g.p = p.dz;
     g.keep = dz;
   }
   if (need_b) {
-    p.dbias = db.mutable_data_ptr();
+    p.dbias = made(db);
     p.bias_dt = bias_type == at::kFloat ? Dt::f32 : dt;
     partial = at::empty({cpd::act_grad_slices(p.m, p.n, dt), n},
                         x.options().dtype(at::kFloat));
-    p.partial = partial.data_ptr<float>();
+    p.partial = made<float>(partial);
   }
   if (need_b || p.dz) cpd::act_grad(p, st);
   // dx: dz [m, n] with W [n, k], the sum runs over n;
@@ -505,14 +526,14 @@ std::vector<Tensor> linear_bwd(const Tensor& dy, const Tensor& x,
     q.b = products.operand(w, true, false, wide, x);
     q.m = (int)m;
     q.k = (int)n;
-    q.y = dx.mutable_data_ptr();
+    q.y = made(dx);
   }
   if (need_w) {
     v.a = products.operand(g, true, padded, wide, x);
     v.b = products.operand(r, true, false, wide, x);
     v.m = (int)n;
     v.k = (int)m;
-    v.y = dw.mutable_data_ptr();
+    v.y = made(dw);
   }
   if (need_x && need_w)
     products.run_two(q, v, x);

@@ -1683,3 +1683,70 @@ def test_gpu_linear_gradients_off_by_one_rounding(dtype, act, m, k, n):
                                  dy.to(dtype).cuda())
     assert times_one_rounding(dx.cpu(), dz @ w, dtype) < 1.2
     assert times_one_rounding(dw.cpu(), dz.t() @ x, dtype) < 1.2
+
+
+class WithoutMemory(torch.Tensor):
+    """A tensor of a wrapper class: on the GPU by its own account, at address
+    0."""
+
+    @staticmethod
+    def __new__(cls, like):
+        return torch.Tensor._make_wrapper_subclass(
+            cls, like.shape, dtype=like.dtype, device="cuda:0")
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise RuntimeError(f"{func} needs memory")
+
+
+def test_refuses_inputs_without_memory():
+    """Before anything is asked of a GPU."""
+    from cpd_amd import ops
+    ext = ops.hip_ext()
+    x = WithoutMemory(torch.zeros(4, 16))
+    t = torch.zeros(4, dtype=torch.int64)
+    for call in (lambda: ext.layer_norm(x, None, None, 1e-5, None),
+                 lambda: ext.linear(x, x, None, 0, None),
+                 lambda: ext.token_logprobs(x, t, 0, -100)):
+        with pytest.raises(TypeError, match="memory"):
+            call()
+
+
+@pytest.mark.gpu
+def test_gpu_refuses_tensors_without_memory():
+    """Every operand, gradients among them, and results: tensors of a wrapper
+    class, zeros known without being stored, a mode that follows shapes
+    alone."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    x = torch.randn(4, 16, device="cuda")
+    w = torch.randn(8, 16, device="cuda")
+    t = torch.zeros(4, dtype=torch.int64, device="cuda")
+    no = WithoutMemory
+    zeros = torch._efficientzerotensor((4, 16), device="cuda")
+    for call in (lambda: fused_layer_norm(zeros),
+                 lambda: fused_layer_norm(x, no(x[0])),
+                 lambda: fused_layer_norm(x, None, no(x[0])),
+                 lambda: fused_layer_norm(x, residual=zeros),
+                 lambda: fused_linear(x, no(w)),
+                 lambda: fused_linear(x, w, no(w[:, 0])),
+                 lambda: fused_linear(x, w, None, "relu", no(x[:, :8])),
+                 lambda: token_logprobs(zeros, t),
+                 lambda: token_logprobs(x, no(t))):
+        with pytest.raises(TypeError, match="memory"):
+            call()
+    for f in (fused_layer_norm, lambda v: fused_linear(v, w, None, "gelu"),
+              lambda v: token_logprobs(v, t).logprobs,
+              lambda v: token_logprobs(v, t).entropy):
+        y = f(x.detach().requires_grad_(True))
+        dy = torch._efficientzerotensor(y.shape, device="cuda")
+        with pytest.raises(TypeError, match="memory"):
+            y.backward(dy)
+    odd = torch.randn(70, 33, device="cuda").bfloat16()
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        for call in (lambda: fused_layer_norm(x), lambda: fused_linear(x, w),
+                     lambda: fused_linear(odd, odd),
+                     lambda: token_logprobs(x, t, 2)):
+            with pytest.raises(TypeError, match="memory"):
+                call()
+    torch.cuda.synchronize()
+    assert torch.isfinite(fused_layer_norm(x)).all()
