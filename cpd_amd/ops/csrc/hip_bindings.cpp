@@ -75,18 +75,20 @@ std::optional<Tensor> learned(const OptTensor& t, const Tensor& x, int64_t n,
       t->scalar_type());
   TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == n, name, " has shape ",
                     t->sizes(), ", wanted [", n, "]");
-  return t->contiguous();
+  return t->resolve_neg().contiguous();
 }
 
 // A tensor as rows of its last axis: itself where the rows are evenly apart
-// and their elements adjacent, a contiguous copy otherwise.
+// and their elements adjacent, a contiguous copy otherwise, and of a view that
+// stands for the negative of what its memory holds (.imag of a conjugate).
 struct Rows {
   Tensor keep;
   const void* p = nullptr;
   long rows = 0, cols = 0, ld = 0;
 };
 
-Rows rows_of(const Tensor& t) {
+Rows rows_of(const Tensor& any) {
+  const Tensor t = any.resolve_neg();
   Rows r;
   r.cols = t.size(-1);
   r.rows = r.cols ? t.numel() / r.cols : 0;
@@ -299,8 +301,8 @@ Tensor logprob_bwd(const Tensor& x, const Tensor& targets, const Tensor& stats,
                         stats.numel() == 2 * r.rows && stats.is_contiguous(),
                     "saved tensors are not these logits'");
   Tensor g, h;
-  if (glp.has_value() && glp->defined()) g = glp->to(at::kFloat).contiguous();
-  if (gent.has_value() && gent->defined()) h = gent->to(at::kFloat).contiguous();
+  if (glp.has_value() && glp->defined()) g = glp->to(at::kFloat).resolve_neg().contiguous();
+  if (gent.has_value() && gent->defined()) h = gent->to(at::kFloat).resolve_neg().contiguous();
   for (const Tensor* v : {&g, &h}) {
     if (v->defined()) check_memory(*v, "a gradient");
     TORCH_CHECK_VALUE(!v->defined() || (v->device() == x.device() &&

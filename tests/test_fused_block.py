@@ -1750,3 +1750,43 @@ def test_gpu_refuses_tensors_without_memory():
                 call()
     torch.cuda.synchronize()
     assert torch.isfinite(fused_layer_norm(x)).all()
+
+
+@on_devices
+def test_negative_views(device):
+    """A view that stands for the negative of its memory, as .imag of a
+    conjugate does, is read as what it stands for: every operand and every
+    incoming gradient."""
+    neg = lambda v: torch._neg_view((-v).contiguous())  # noqa: E731
+    g = rng(91)
+    draw = lambda *s: normal(  # noqa: E731
+        g, *s, dtype=torch.float32, device=device)
+    x, res, w, b = draw(6, 16), draw(6, 16), draw(16, 16), draw(16)
+    dy, dz, t = draw(6, 16), draw(6), torch.arange(6, device=device)
+    c = torch.randn(6, 1, generator=g, dtype=torch.complex64).to(
+        device).conj().imag
+    assert c.is_neg() and neg(x).is_neg() and torch.equal(neg(x), x)
+    one = torch.ones(1, 1, device=device)
+    assert torch.equal(fused_linear(c, one), c.clone())
+
+    def norm(x, res, w, b, dy, dz):
+        y, s = fused_layer_norm(x, w[0], b, residual=res)
+        return y, s, *torch.autograd.grad([y, s], [x, res, w, b], [dy, dy])
+
+    def linear(x, res, w, b, dy, dz):
+        y = fused_linear(x, w, b, "gelu", res)
+        return y, *torch.autograd.grad(y, [x, w, b, res], dy)
+
+    def logprobs(x, res, w, b, dy, dz):
+        out = token_logprobs(x, t, 3)
+        return *out, *torch.autograd.grad([out.logprobs, out.entropy], x,
+                                          [dz, dz])
+
+    for f in (norm, linear, logprobs):
+        plain, negated = ([v.detach().requires_grad_(True) for v in ops] +
+                          list(grads) for ops, grads in (
+            ((x, res, w, b), (dy, dz)),
+            (map(neg, (x, res, w, b)), (neg(dy), neg(dz)))))
+        assert all(v.is_neg() for v in negated)
+        assert all(torch.equal(p, q)
+                   for p, q in zip(f(*negated), f(*plain)))
