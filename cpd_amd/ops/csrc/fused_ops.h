@@ -49,7 +49,7 @@ struct LogprobArgs {
   const int64_t* targets;   // [rows]
   float* logprobs;          // [rows]
   float* entropy;           // [rows]
-  float* stats;             // [rows, 2]: maximum, log of the sum around it
+  float* stats;             // [rows, 2]: maximum, sum around it
   int64_t* top_ids;         // [rows, top] or null
   float* top_logprobs;      // [rows, top] or null
   void* work;               // logprob_work_bytes(), 8-byte aligned

@@ -1790,3 +1790,24 @@ def test_negative_views(device):
         assert all(v.is_neg() for v in negated)
         assert all(torch.equal(p, q)
                    for p, q in zip(f(*negated), f(*plain)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab", [(64, 131072), (600, 50021), (40, 4096),
+                                        (900, 1000)])
+def test_gpu_logprobs_probabilities_as_exact_as_floats_are(rows, vocab):
+    """The gradient of a log probability is minus the others' probabilities,
+    e^(x - max) over its sum.  Each is off by the rounding of x - max (|x - max|
+    between 8 and 16: up to 8 U, 4.6 U root mean square; the more so the less
+    often), of e^, of its product and of the sum (1, 1 and at most 3 U).  Taken
+    from the rounded log probability it would be 10 to 20 U, so 9 U are
+    allowed."""
+    g = rng(rows, vocab, 19)
+    x = torch.randn(rows, vocab, generator=g) * 3
+    t = torch.zeros(rows, dtype=torch.int64)
+    leaf = x.cuda().requires_grad_(True)
+    out = token_logprobs(leaf, t.cuda())
+    dx, = torch.autograd.grad(out.logprobs.sum(), leaf)
+    p = torch.softmax(leaf.detach().double(), -1)[:, 1:]
+    off = (-dx[:, 1:].double() - p) / p
+    assert off.square().mean().sqrt() < 9 * U
