@@ -76,6 +76,20 @@ struct Soft {  // running maximum and sums
   float m, s, a;
 };
 
+// Two by two, so that no term is rounded more than log2 N times.
+template <int N>
+__device__ __forceinline__ float sum_of(const float* v) {
+  if constexpr (N == 1) return v[0];
+  else return sum_of<N / 2>(v) + sum_of<N / 2>(v + N / 2);
+}
+
+// Adds x to a sum that is the larger of the two; what that loses goes to `low`.
+__device__ __forceinline__ void add_to(float& sum, float& low, float x) {
+  const float t = sum + x;
+  low += (sum - t) + x;
+  sum = t;
+}
+
 // The sums of `o` and `v`, around the larger maximum.
 __device__ __forceinline__ Soft join(Soft v, Soft o) {
   const float m = fmaxf(v.m, o.m);
@@ -366,6 +380,10 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int parts,
     const int to = a.vocab - from < per ? a.vocab : from + per;
     const T* x = static_cast<const T*>(a.x) + row * a.ld;
     Soft v = {-INFINITY, 0.f, 0.f};
+    // What the sums' roundings lost: a lane adds hundreds of small terms to the 1
+    // that a row's maximum is (131072 floats, one of them at 0 and the rest at -12:
+    // S was 1e-5 off without).
+    float low_s = 0.f, low_a = 0.f;
     // Values below `bar` need not be kept.  (k of them are from it on, and those
     // of this wave's that equal it and come later come after them.)
     float bar = -INFINITY;
@@ -383,18 +401,25 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int parts,
         const float f = v.m == -INFINITY ? 0.f : fast_exp(d);
         v.a = f * (v.a + d * v.s);
         v.s *= f;
+        low_a = f * (low_a + d * low_s);
+        low_s *= f;
         v.m = big;
       }
       const float about = v.m == -INFINITY ? 0.f : v.m;
+      float some_s[LOADS], some_a[LOADS];
 #pragma unroll
-      for (int c = 0; c < LOADS; ++c)
+      for (int c = 0; c < LOADS; ++c) {
+        some_s[c] = some_a[c] = 0.f;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           const float d = as_float(u[c][i]) - about;
           const float e = fast_exp(d);
-          v.s += e;
-          v.a += e * near(d);
+          some_s[c] += e;
+          some_a[c] += e * near(d);
         }
+      }
+      add_to(v.s, low_s, sum_of<LOADS>(some_s));
+      add_to(v.a, low_a, sum_of<LOADS>(some_a));
       if (!TOP) return;
       // a NaN is passed over by the maximum, but it makes the sum one
       const bool odd = v.s != v.s;
@@ -464,6 +489,8 @@ __global__ __launch_bounds__(256) void logprob_kernel(LogprobArgs a, int parts,
       work(base, u);
     }
     if (TOP) settle(top, pendings[wave], count);
+    v.s += low_s;
+    v.a += low_a;
     v = wave_join(v);
     if (WAVES > 1) block_join<WAVES, TOP>(v, top, softs, lists);
     if (tid < 64) {

@@ -1811,3 +1811,26 @@ def test_gpu_logprobs_probabilities_as_exact_as_floats_are(rows, vocab):
     p = torch.softmax(leaf.detach().double(), -1)[:, 1:]
     off = (-dx[:, 1:].double() - p) / p
     assert off.square().mean().sqrt() < 9 * U
+
+
+@pytest.mark.gpu
+@on_types
+@pytest.mark.parametrize("rows", [3, 520])
+@pytest.mark.parametrize("rest", [-11.5, -11.9375, -12.0, -12.6875])
+def test_gpu_logprobs_many_small_terms(dtype, rows, rest):
+    """One entry far above 131071 equal ones, each of which is some tenths of a
+    step of the sum that it is added to: what one addition loses all lose, so it
+    has to be kept.  Off by: a step's 32 additions, 10 joins, e^'s own |rest| + 4;
+    the logarithm and its differences 4: 64 U cover S, for the entropy |rest|
+    times that beside it."""
+    vocab = 131072
+    x = torch.full((rows, vocab), rest, dtype=dtype, device="cuda")
+    t = torch.arange(rows, device="cuda") * 97 % vocab
+    x[torch.arange(rows, device="cuda"), t] = 0.0
+    out = token_logprobs(x, t, 2)
+    small = (vocab - 1) * math.exp(rest)
+    logs = math.log1p(small)
+    ent = logs - small * rest / (1 + small)
+    assert (out.logprobs.double() + logs).abs().max() < 64 * U
+    assert (out.entropy.double() - ent).abs().max() < 64 * U * (1 - rest)
+    assert torch.equal(out.top_ids[:, 0], t)
