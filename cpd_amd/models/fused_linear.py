@@ -72,8 +72,7 @@ def fused_linear(x, weight, bias=None, activation=None, residual=None):
     multiplications, or 2^24 weights) and 16-bit, the gradient behind the
     activation is rounded to that type too.  Of float32 operands (the inputs
     and, backward, the incoming gradient) the GPU may leave out what lies below
-    2^-133: that of forward depends on the number of rows and the weight's
-    size, that of both gradients does not.
+    2^-133, depending on the sizes.
 
     Rows may be apart by any stride; the result is contiguous.  Raises
     TypeError and ValueError for types and shapes that do not fit.

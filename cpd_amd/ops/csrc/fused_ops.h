@@ -77,6 +77,10 @@ struct LogprobGradArgs {
 void logprob_backward(const LogprobGradArgs& a, hipStream_t stream);
 
 enum class Act : int { none = 0, relu = 1, gelu = 2, silu = 3 };
+// Which kernel makes a product: tiles; few rows of A, both operands along, straight
+// from memory; floats with few rows of B or of A; short sums of floats (`tile`: the
+// rows that a wave goes down).
+enum class Way : int { tiles = 0, rows = 1, narrow_b = 2, narrow_a = 3, brief = 4 };
 
 // C[m, n] = sum over k of A(m, k) B(n, k), and what becomes of it.  An operand
 // lies with k innermost (A[m * ld + k]) or, `across`, with k outermost
@@ -101,7 +105,8 @@ struct GemmArgs {
   long res_ld;
   Act act;
   float* work;        // gemm_work() floats
-  int tile, slices;   // how it is cut up, by gemm_plan
+  Way way;            // how it is cut up, by gemm_plan
+  int tile, slices;
 };
 // Sets how a product is cut up, from its sizes and layouts.
 void gemm_plan(GemmArgs& g);

@@ -548,9 +548,9 @@ std::vector<Tensor> linear_bwd(const Tensor& dy, const Tensor& x,
 }
 
 // How the products of m rows, n features out and k in are cut up (without an
-// activation): tile and slices of forward, of dx and of dW, and whether a call
-// for both gradients takes one launch.  Which kernels run is not seen in the
-// results, and tests have to reach every one.
+// activation): tile and slices of forward, of dx and of dW, whether a call for
+// both gradients takes one launch, and the three products' way.  Which kernels run
+// is not seen in the results, and tests have to reach every one.
 std::vector<int64_t> linear_plan(int64_t m, int64_t n, int64_t k,
                                  at::ScalarType type, bool need_x, bool need_w) {
   check_sizes(m, n, k);
@@ -577,7 +577,8 @@ std::vector<int64_t> linear_plan(int64_t m, int64_t n, int64_t k,
     cpd::gemm_plan(dx);
     cpd::gemm_plan(dw);
   }
-  return {y.tile, y.slices, dx.tile, dx.slices, dw.tile, dw.slices, together};
+  return {y.tile,    y.slices,   dx.tile,     dx.slices,   dw.tile,
+          dw.slices, together, (int)y.way, (int)dx.way, (int)dw.way};
 }
 
 // ---------------------------------------------------------------------------
@@ -743,7 +744,8 @@ void cpd_register_fused(pybind11::module_& m) {
   m.def("layer_norm", &layer_norm, "layer norm (+residual): [y] or [y, s]");
   m.def("linear", &linear, "act(x W^T + bias) + residual");
   m.def("linear_plan", &linear_plan,
-        "[tile, slices] of y, dx and dW, and whether the last two share a launch");
+        "[tile, slices] of y, dx and dW, whether the last two share a launch, "
+        "and the way of each");
   m.def("token_logprobs", &token_logprobs,
         "[logprobs, entropy] or [logprobs, entropy, top_ids, top_logprobs]");
 }

@@ -593,8 +593,9 @@ gemm_two_kernel(GemmArgs dx, GemmArgs dw, int first, bool dw_first) {
 // 134 MB of 16-bit B (k 4096, k 16384, k 5000) 1 row takes 26, 29 and 34 us, 16
 // take 28, 32 and 43, 32 take 36, 39 and 55, and by tiles of 128 16 take 34, 34
 // and 41, 32 take 31, 33 and 42; with 34 MB 16 take 10, 32 take 14 and by tiles 15;
-// with 8 MB 32 and 48 took 7 and 9, by tiles 14.  With 134 MB of floats 32 take 48,
-// by tiles 54.
+// with 8 MB 32 and 48 took 7 and 9, by tiles 14.  Floats of more than 16 MB go to
+// gemm_narrow_kernel: with 134 MB 1, 16 and 32 rows take 30, 31 and 35 there, 32, 37
+// and 48 here, and by tiles 32 take 54.
 template <typename T, int F, int W>
 __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g) {
   constexpr int VEC = 16 / sizeof(T);    // a lane's elements of a load
@@ -714,6 +715,262 @@ __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g) {
   }
 }
 
+// Few features of floats: a block has ROWS rows of one operand ("many") by all of
+// at most 16 F of the other ("few"), so that many is read once, and multiplies them
+// by the float matrix instructions (a tile of 128 by 128 would be cut into parts
+// and multiplied for the few columns that it has).  A tile is 4096 / ROWS of k.
+// Its 512 threads read three tiles ahead into registers and write to LDS, which has
+// two; its eight waves have 16 rows and 32 k of a tile each, and add up through LDS.
+// A fragment's eight k are 8 (lane / 16) and on: adjacent in LDS if the operand
+// lies along, its chunks swizzled; RS + 2 apart if across, which keeps the four
+// groups of lanes off each other's banks.
+//
+// Bound by reading many: 590 MB, 16384 x 9000 to 8, take 103 us forward and 110 for
+// dW (5.7 and 5.4 TB/s; by tiles 182 and 202).
+template <int RS, int K, bool ACROSS>
+struct NarrowStager {  // a thread's share of RS rows by K k
+  static constexpr int CHUNKS = RS * K / 4;
+  static constexpr int PASSES = (CHUNKS + 511) / 512;
+  static constexpr int BYTES = ACROSS ? K * (RS + 2) * 4 : RS * K * 4;
+  const float* p[PASSES];
+  int at[PASSES];   // this thread's first k in a tile, or its k
+  u32 place[PASSES];
+  long step;
+  int rows_left[PASSES];  // across: rows from its first on
+  bool on;
+
+  __device__ __forceinline__ void start(const Operand& o, int row0, int rows, int tid) {
+    const float* base = static_cast<const float*>(o.p);
+    on = tid < CHUNKS;  // (or CHUNKS is a multiple of 512)
+    step = ACROSS ? K * o.ld : K;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int id = tid + 512 * i;
+      if constexpr (!ACROSS) {
+        const int r = id / (K / 4), chunk = id % (K / 4);
+        at[i] = chunk * 4;
+        rows_left[i] = 4;
+        // (rows behind the last one repeat it: their results are not stored)
+        p[i] = base + (long)min(row0 + r, rows - 1) * o.ld + at[i];
+        place[i] = r * (K * 4) + ((chunk ^ (r & 7)) << 4);
+      } else {
+        const int chunk = id % (RS / 4);
+        at[i] = id / (RS / 4);
+        rows_left[i] = rows - (row0 + chunk * 4);
+        p[i] = base + (long)at[i] * o.ld + row0 + chunk * 4;
+        place[i] = (at[i] * (RS + 2) + chunk * 4) * 4;
+      }
+    }
+  }
+  // `left`: k from this tile's first on
+  __device__ __forceinline__ void load(int tile, int left, float (&v)[PASSES][4]) const {
+    if (!on) return;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i)
+      load_some<float, 4>(p[i] + tile * step,
+                          ACROSS ? (at[i] < left ? rows_left[i] : 0) : left - at[i],
+                          v[i]);
+  }
+  __device__ __forceinline__ void store(char* lds, const float (&v)[PASSES][4]) const {
+    if (!on) return;
+    typedef float V __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      if constexpr (!ACROSS) {
+        *reinterpret_cast<f32x4*>(lds + place[i]) =
+            f32x4{v[i][0], v[i][1], v[i][2], v[i][3]};
+      } else {
+        *reinterpret_cast<V*>(lds + place[i]) = V{v[i][0], v[i][1]};
+        *reinterpret_cast<V*>(lds + place[i] + 8) = V{v[i][2], v[i][3]};
+      }
+    }
+  }
+  // 16 rows from `row`, 32 k from `k`
+  static __device__ __forceinline__ void fragment(const char* lds, int row, int k, int lane,
+                                                  float (&v)[8]) {
+    const int r = row + (lane & 15), group = lane >> 4;
+    if constexpr (!ACROSS) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x4 u = *reinterpret_cast<const f32x4*>(
+            lds + r * (K * 4) + (((k / 4 + group * 2 + h) ^ (r & 7)) << 4));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[h * 4 + i] = u[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = *reinterpret_cast<const float*>(lds + ((k + group * 8 + i) * (RS + 2) + r) * 4);
+    }
+  }
+};
+
+// MX, FX: many, few lie across.  MANY_A: many is A, otherwise B.
+template <int F, int ROWS, bool MX, bool FX, bool MANY_A>
+__global__ __launch_bounds__(512) void gemm_narrow_kernel(GemmArgs g) {
+  constexpr int K = 4096 / ROWS, GROUPS = ROWS / 16, SHARES = 8 / GROUPS;
+  using Many = NarrowStager<ROWS, K, MX>;
+  using Few = NarrowStager<16 * F, K, FX>;
+  constexpr int BUF = Many::BYTES + Few::BYTES;
+  __shared__ __attribute__((aligned(16))) char lds[2 * BUF];
+  static_assert(2 * BUF >= 8 * F * 1024, "sums through LDS");
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int many = MANY_A ? g.m : g.n, few = MANY_A ? g.n : g.m;
+  const int blocks = (many + ROWS - 1) / ROWS;
+  const int slice = blockIdx.x / blocks, row0 = blockIdx.x % blocks * ROWS;
+  const int all = (g.k + K - 1) / K;
+  const int per = (all + g.slices - 1) / g.slices;
+  const int from = min(slice * per, all), to = min(from + per, all);
+  const int mine = wave % GROUPS * 16, share = wave / GROUPS;
+  Many sm;
+  Few sf;
+  sm.start(MANY_A ? g.a : g.b, row0, many, threadIdx.x);
+  sf.start(MANY_A ? g.b : g.a, 0, few, threadIdx.x);
+  f32x4 acc[F] = {};
+  struct Raw {
+    float m[Many::PASSES][4], f[Few::PASSES][4];
+  };
+  // (blocks begin at different k, as in gemm_rows_kernel: 12 x 16384 to 16384 took
+  // 225 us with all from their first on)
+  const bool apart = !MX && ((MANY_A ? g.a : g.b).ld * 4) % 4096 == 0 && to > from;
+  const int turn = apart ? (int)(blockIdx.x * 5) % (to - from) : 0;
+  auto load = [&](int t, Raw& r) {
+    if (t >= to) return;
+    const int k = t + turn < to ? t + turn : t + turn - (to - from);
+    sm.load(k, g.k - k * K, r.m);
+    sf.load(k, g.k - k * K, r.f);
+  };
+  auto step = [&](int t, Raw& r) {
+    if (t >= to) return;
+    // (tile t - 2, whose place this takes, was read before the last barrier)
+    char* buf = lds + ((t - from) & 1) * BUF;
+    sm.store(buf, r.m);
+    sf.store(buf + Many::BYTES, r.f);
+    load(t + 3, r);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (loads stay in flight)
+    block_barrier();
+    float vm[8], vf[F][8];
+    Many::fragment(buf, mine, share * 32, lane, vm);
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+      Few::fragment(buf + Many::BYTES, f * 16, share * 32, lane, vf[f]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int f = 0; f < F; ++f)
+        // (a lane gets four neighbouring columns of the result)
+        acc[f] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+            MANY_A ? vf[f][i] : vm[i], MANY_A ? vm[i] : vf[f][i], acc[f], 0, 0, 0);
+  };
+  Raw r0, r1, r2;
+  load(from, r0);
+  load(from + 1, r1);
+  load(from + 2, r2);
+  for (int t = from; t < to; t += 3) {
+    step(t, r0);
+    step(t + 1, r1);
+    step(t + 2, r2);
+  }
+  if constexpr (SHARES > 1) {
+    __syncthreads();  // the tiles have been read
+    f32x4* sums = reinterpret_cast<f32x4*>(lds);
+#pragma unroll
+    for (int f = 0; f < F; ++f) sums[(wave * F + f) * 64 + lane] = acc[f];
+    __syncthreads();
+    if (share > 0) return;
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+      for (int q = 1; q < SHARES; ++q)
+        acc[f] += sums[((wave + q * GROUPS) * F + f) * 64 + lane];
+  }
+#pragma unroll
+  for (int f = 0; f < F; ++f) {
+    const int row = (MANY_A ? row0 + mine : f * 16) + (lane & 15);
+    const int col = (MANY_A ? f * 16 : row0 + mine) + (lane >> 4) * 4;
+    float v[4] = {acc[f][0], acc[f][1], acc[f][2], acc[f][3]}, bias[4] = {};
+    if (g.slices > 1) {
+      if (row < g.m && col < g.n)
+        store_some<float, 4>(g.work + ((long)slice * g.m + row) * g.n + col, g.n - col, v);
+      continue;
+    }
+    if (g.bias) load_learned<4>(g.bias, g.bias_dt, col, g.n - col, bias);
+    finish<float, 4>(g, row, col, v, bias);
+  }
+}
+
+// Sums of at most 16 Q floats: bound by writing the result.  A wave keeps 64 of B's
+// rows in registers and goes down `rows_per` rows of A, sixteen at a time, the next
+// ones in flight; it has no LDS and no barrier, so that waves write while others
+// load.  A lane's elements of a sum are 4 Q (lane / 16) and on.  16384 x 9000 out of
+// sums of 8, 590 MB: 190 us (by tiles 245).
+template <int Q, bool AX, bool BX>
+__global__ __launch_bounds__(256) void gemm_short_kernel(GemmArgs g, int rows_per) {
+  constexpr int N = 4 * Q;
+  const int lane = threadIdx.x & 63;
+  const int wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int strips = (g.n + 63) / 64;
+  const int col0 = wave % strips * 64;
+  const long first = (long)(wave / strips) * rows_per;
+  if (first >= g.m) return;
+  const int from = (int)first, to = min(g.m - from, rows_per) + from;
+  const int k0 = (lane >> 4) * N;
+  float b[4][N], bias[4][4] = {};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    // (rows behind the last one repeat it: their results are not stored)
+    const long row = min(col0 + w * 16 + (lane & 15), g.n - 1);
+    if constexpr (BX) {
+      const float* p = static_cast<const float*>(g.b.p) + (long)k0 * g.b.ld + row;
+#pragma unroll
+      for (int i = 0; i < N; ++i) b[w][i] = k0 + i < g.k ? p[i * g.b.ld] : 0.f;
+    } else {
+      const float* p = static_cast<const float*>(g.b.p) + row * g.b.ld + k0;
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+        load_some<float, 4>(p + 4 * q, g.k - k0 - 4 * q, &b[w][4 * q]);
+    }
+    const int col = col0 + w * 16 + (lane >> 4) * 4;
+    if (g.bias) load_learned<4>(g.bias, g.bias_dt, col, g.n - col, bias[w]);
+  }
+  auto load = [&](int row, float (&a)[N]) {
+    const long mine = min(row + (lane & 15), g.m - 1);
+    if constexpr (AX) {
+      const float* p = static_cast<const float*>(g.a.p) + (long)k0 * g.a.ld + mine;
+#pragma unroll
+      for (int i = 0; i < N; ++i) a[i] = k0 + i < g.k ? p[i * g.a.ld] : 0.f;
+    } else {
+      const float* p = static_cast<const float*>(g.a.p) + mine * g.a.ld + k0;
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+        load_some<float, 4>(p + 4 * q, g.k - k0 - 4 * q, &a[4 * q]);
+    }
+  };
+  auto work = [&](int row, const float (&a)[N]) {
+    f32x4 acc[4] = {};
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        acc[w] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[w][i], a[i], acc[w], 0, 0, 0);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      float v[4] = {acc[w][0], acc[w][1], acc[w][2], acc[w][3]};
+      finish<float, 4>(g, row + (lane & 15), col0 + w * 16 + (lane >> 4) * 4, v, bias[w]);
+    }
+  };
+  float a0[N], a1[N];
+  load(from, a0);
+  for (int row = from; row < to; row += 32) {
+    if (row + 16 < to) load(row + 16, a1);
+    work(row, a0);
+    if (row + 16 >= to) break;
+    if (row + 32 < to) load(row + 32, a0);
+    work(row + 16, a1);
+  }
+}
+
 // The slices' sums, in order, and what follows the product.
 template <typename T>
 __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs g) {
@@ -739,11 +996,19 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs g) {
 // Whether gemm_rows_kernel takes a product of operands along (its figures).
 bool gemm_few_rows(long m, long n, long k, Dt dt) {
   const long bytes = n * k * dt_size(dt);
-  return m <= 16 || (m <= 32 && (dt == Dt::f32 || bytes <= (48L << 20))) ||
-         (m <= 64 && bytes <= (16L << 20));
+  if (m <= 64 && bytes <= (16L << 20)) return true;
+  // (floats of up to 32 rows otherwise: few features, with less time)
+  return dt != Dt::f32 && (m <= 16 || (m <= 32 && bytes <= (48L << 20)));
 }
 
 namespace {
+
+// Up to how many rows or features of floats are few.  (Kernels of a pass forward and
+// backward without bias, by 128-tiles and as few, us: 16384 x 5000 to 17 349 and 280,
+// 16384 x 8 to 9000 653 and 426, 4000 x 10000 to 10 185 and 131, 4 x 12608 to 11709
+// 617 and 397, 1152 x 1088 to 25 33 and 30.  From 33 on a step with bias took longer:
+// 8192 x 48 to 4096 182 and 211, 16384 x 2048 to 64 168 and 182.)
+constexpr int kFew = 32;
 
 // How a product is cut up, and the time that it takes.  The tile kernels have
 // one block a CU, so time goes by rounds of 256 blocks.  In units of a 128-tile's
@@ -809,8 +1074,18 @@ void take(GemmArgs& g, const Plan& p) {
 }
 
 unsigned blocks_of(const GemmArgs& g) {
-  const int tm = g.tile < 128 ? 1 : (g.m + g.tile - 1) / g.tile;
-  return (unsigned)(tm * ((g.n + g.tile - 1) / g.tile) * g.slices);
+  const int tm = (g.m + g.tile - 1) / g.tile, tn = (g.n + g.tile - 1) / g.tile;
+  switch (g.way) {
+    case Way::brief:  // four waves a block
+      return (unsigned)(((long)tm * ((g.n + 63) / 64) + 3) / 4);
+    case Way::rows:
+    case Way::narrow_a:
+      return (unsigned)(tn * g.slices);
+    case Way::narrow_b:
+      return (unsigned)(tm * g.slices);
+    default:
+      return (unsigned)(tm * tn * g.slices);
+  }
 }
 
 template <typename O>
@@ -828,11 +1103,50 @@ void gemm_tiles_t(const GemmArgs& g, hipStream_t st) {
     if constexpr (!__is_same(T, float) && BX)
       gemm_kernel<T, AX, BX, kWide>
           <<<grid, dim3(kThreads<T, kWide>), 0, st>>>(g);
-  } else if (g.tile == 256) {
-    if constexpr (!__is_same(T, float))
+  } else if (g.way == Way::tiles) {
+    if (g.tile == 128) {
+      gemm_kernel<T, AX, BX, 128><<<grid, threads, 0, st>>>(g);
+    } else if constexpr (!__is_same(T, float)) {
       gemm_kernel<T, AX, BX, 256><<<grid, threads, 0, st>>>(g);
-  } else if (g.tile == 128) {
-    gemm_kernel<T, AX, BX, 128><<<grid, threads, 0, st>>>(g);
+    }
+  } else if (g.way == Way::brief) {
+    if constexpr (__is_same(T, float)) {
+      auto start = [&](auto q) {
+        gemm_short_kernel<decltype(q)::value, AX, BX>
+            <<<grid, dim3(256), 0, st>>>(g, g.tile);
+      };
+      using std::integral_constant;
+      g.k <= 16 ? start(integral_constant<int, 1>()) : start(integral_constant<int, 2>());
+    }
+  } else if (g.way == Way::narrow_a || g.way == Way::narrow_b) {
+    if constexpr (__is_same(T, float)) {
+      using std::integral_constant;
+      auto start = [&](auto f) {
+        constexpr int F = decltype(f)::value;
+        // (many lies across: 32 or 128 rows of it a block; along: 32)
+        auto block = [&](auto rows, auto many_a) {
+          constexpr bool MANY_A = decltype(many_a)::value;
+          gemm_narrow_kernel<F, decltype(rows)::value, MANY_A ? AX : BX,
+                             MANY_A ? BX : AX, MANY_A>
+              <<<grid, dim3(512), 0, st>>>(g);
+        };
+        const integral_constant<int, 32> few_rows;
+        const integral_constant<int, 128> rows;
+        if (g.way == Way::narrow_b) {
+          if constexpr (AX) {
+            if (g.tile == 128) return block(rows, std::true_type{});
+          }
+          block(few_rows, std::true_type{});
+        } else {
+          if constexpr (BX) {
+            if (g.tile == 128) return block(rows, std::false_type{});
+          }
+          block(few_rows, std::false_type{});
+        }
+      };
+      const int few = g.way == Way::narrow_b ? g.n : g.m;
+      few <= 16 ? start(integral_constant<int, 1>()) : start(integral_constant<int, 2>());
+    }
   } else if constexpr (!AX && !BX) {
     auto start = [&](auto f, auto w) {
       gemm_rows_kernel<T, decltype(f)::value, decltype(w)::value>
@@ -842,13 +1156,13 @@ void gemm_tiles_t(const GemmArgs& g, hipStream_t st) {
     const integral_constant<int, 1> one;
     const integral_constant<int, 2> two;
     const integral_constant<int, 4> four;
-    if (g.tile == 32) {
-      if constexpr (__is_same(T, float))
-        g.m <= 16 ? start(one, two) : start(two, two);
-      else
-        start(one, two);  // (more rows go to tiles: gemm_few_rows)
-    } else
+    auto sixteen = [&] {
       g.m <= 16 ? start(one, one) : g.m <= 32 ? start(two, one) : start(four, one);
+    };
+    if constexpr (__is_same(T, float))
+      sixteen();  // (plan_rows: more than 48 MB of floats go elsewhere)
+    else
+      g.tile == 32 ? start(one, two) : sixteen();
   }
   join_slices<T>(g, st);
 }
@@ -997,33 +1311,84 @@ void gemm_two(const GemmArgs& dx, const GemmArgs& dw, hipStream_t st) {
     gemm_two_tiles<f16_t>(dx, dw, st);
 }
 
+namespace {
+
+void plan_tiles(GemmArgs& g) {
+  double least = INFINITY;
+  each_plan(g, false, [&](const Plan& p) {
+    if (time_of(p) >= least) return;
+    least = time_of(p);
+    take(g, p);
+  });
+}
+
+// A product for gemm_rows_kernel.
+void plan_rows(GemmArgs& g) {
+  // 16 rows of B a block, or 32 where A would be read too often (1 row with 134
+  // MB and k 5000: 34 us, with 16 of B 43; with 34 MB 16 are faster)
+  const long bytes = (long)g.n * g.k * dt_size(g.dt);
+  g.way = Way::rows;
+  g.tile = bytes > (48L << 20) ? 32 : 16;  // (at most 16 rows then)
+  const long blocks = (g.n + g.tile - 1) / g.tile;
+  const long lines = (long)g.k * dt_size(g.dt) / 128;
+  long s = 512 / blocks;  // two blocks a CU, eight lines a wave at least
+  if (s > lines / 64) s = lines / 64;
+  g.slices = (int)(s < 1 ? 1 : s > 32 ? 32 : s);
+}
+
+// Floats with few rows or columns and with short sums; whether this is one.
+bool plan_few(GemmArgs& g) {
+  if (g.dt != Dt::f32) return false;
+  // The gradients of a layer this small take one launch of tiles together (a whole
+  // step of 3 x 16 to 19: 62 us, 67 with two launches, most of it the host's).
+  if (g.b.across && g.m <= 128 && g.n <= 128 && g.k <= 128) return false;
+  if (g.k <= kFew) {
+    g.way = Way::brief;
+    // rows of A that a wave goes down: eight waves a SIMD, if there are as many
+    const long strips = (g.n + 63) / 64, groups = (g.m + 15L) / 16;
+    long chunks = 8192 / strips;
+    chunks = chunks < 1 ? 1 : chunks > groups ? groups : chunks;
+    g.tile = (int)((groups + chunks - 1) / chunks) * 16;
+    return true;
+  }
+  const bool a = g.m <= kFew, b = g.n <= kFew && (!a || g.n <= g.m);
+  if (!a && !b) return false;
+  const long many = b ? g.m : g.n;
+  if (many > 1L << 27) return false;  // (a launch holds less than 2^32 threads)
+  g.way = b ? Way::narrow_b : Way::narrow_a;
+  // 32 rows of many a block; where it lies across those are 128 bytes of a row of
+  // memory, so 128 if there are blocks enough (4000 x 10000 to 10: dW 35 us, with 32
+  // 49; 2000 x 4096 to 32: 16 and 15, 512 x 2048 to 10 10 and 5)
+  const bool across = b ? g.a.across : g.b.across;
+  g.tile = across && many > 4608 ? 128 : 32;
+  const long blocks = (many + g.tile - 1) / g.tile;
+  const long tiles = ((long)g.k * g.tile + 4095) / 4096;
+  // two blocks a CU, twelve tiles each at least: the joining kernel is another
+  // launch and 4 us (512 x 2048 to 10 forward, 16 tiles: 11.3 us in one slice, 9.6 in
+  // two; 3000 x 25 to 700 dW, 24 tiles: 33 in one, 17 in three)
+  long s = 512 / blocks;
+  if (s > tiles / 12) s = tiles / 12;
+  g.slices = (int)(s < 1 ? 1 : s > 32 ? 32 : s);
+  return true;
+}
+
+}  // namespace
+
 void gemm_plan(GemmArgs& g) {
+  g.way = Way::tiles;
   g.tile = 128;
   g.slices = 1;
   if (g.m < 1 || g.n < 1) return;  // nothing will be launched
-  if (!g.a.across && !g.b.across && gemm_few_rows(g.m, g.n, g.k, g.dt)) {
-    // 16 rows of B a block, or 32 where A would be read too often (1 row with 134
-    // MB and k 5000: 34 us, with 16 of B 43; with 34 MB 16 are faster)
-    const long bytes = (long)g.n * g.k * dt_size(g.dt);
-    g.tile = g.m <= 32 && bytes > (48L << 20) ? 32 : 16;
-    const long blocks = (g.n + g.tile - 1) / g.tile;
-    const long lines = (long)g.k * dt_size(g.dt) / 128;
-    long s = 512 / blocks;  // two blocks a CU, eight lines a wave at least
-    if (s > lines / 64) s = lines / 64;
-    g.slices = (int)(s < 1 ? 1 : s > 32 ? 32 : s);
-  } else {
-    double least = INFINITY;
-    each_plan(g, false, [&](const Plan& p) {
-      if (time_of(p) >= least) return;
-      least = time_of(p);
-      take(g, p);
-    });
-  }
+  if (!g.a.across && !g.b.across && gemm_few_rows(g.m, g.n, g.k, g.dt))
+    plan_rows(g);
+  else if (!plan_few(g))
+    plan_tiles(g);
 }
 
 bool gemm_plan_two(GemmArgs& a, GemmArgs& b) {
   gemm_plan(a);
   gemm_plan(b);
+  if (a.way != Way::tiles || b.way != Way::tiles) return false;
   // (where both fill their rounds two launches are not slower: 2048^3 of bf16
   // took 45 us in two, 48 in one)
   double least = time_of(plan_of(a, a.tile, a.slices)) +

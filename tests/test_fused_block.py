@@ -1834,3 +1834,127 @@ def test_gpu_logprobs_many_small_terms(dtype, rows, rest):
     assert (out.logprobs.double() + logs).abs().max() < 64 * U
     assert (out.entropy.double() - ent).abs().max() < 64 * U * (1 - rest)
     assert torch.equal(out.top_ids[:, 0], t)
+
+
+TILES, ROWS, NARROW_B, NARROW_A, BRIEF = range(5)
+
+
+# Floats with few features in or out and few rows: up to 16, up to 32 and one
+# more; long sums in one slice and in several; the long operand read 32 or 128
+# rows at a time; rows of it a multiple of 4 KB apart or not; sizes that end inside
+# a vector, a tile and a strip of 64.  (way of y, of dx, of dW)
+FEW_SHAPES = [
+    (70, 300, 9, (NARROW_B, BRIEF, NARROW_A)),
+    (200, 9, 301, (BRIEF, NARROW_B, NARROW_B)),
+    (131, 32, 400, (BRIEF, NARROW_B, NARROW_B)),
+    (131, 33, 400, (TILES, TILES, TILES)),
+    (300, 1025, 31, (NARROW_B, BRIEF, NARROW_A)),
+    (300, 1030, 33, (TILES, TILES, TILES)),
+    (70, 9001, 20, (NARROW_B, BRIEF, NARROW_A)),
+    (70, 4096, 16, (NARROW_B, BRIEF, NARROW_A)),
+    (5003, 200, 7, (NARROW_B, BRIEF, NARROW_A)),
+    (5003, 18, 201, (BRIEF, NARROW_B, NARROW_B)),
+    (700, 4700, 9, (NARROW_B, BRIEF, NARROW_A)),
+    (700, 25, 4703, (BRIEF, NARROW_B, NARROW_B)),
+    (3000, 4610, 17, (NARROW_B, BRIEF, NARROW_A)),
+    (20, 300, 5000, (ROWS, NARROW_A, BRIEF)),
+    (3, 4900, 1003, (NARROW_A, NARROW_A, BRIEF)),
+    (17, 4096, 1100, (NARROW_A, NARROW_A, BRIEF)),
+    (32, 5000, 900, (NARROW_A, NARROW_A, BRIEF)),
+    (1, 150, 1, (ROWS, BRIEF, BRIEF)),
+    (129, 1, 1, (BRIEF, BRIEF, NARROW_B)),
+    (9, 20, 30, (ROWS, TILES, TILES)),
+    (128, 128, 20, (NARROW_B, TILES, TILES)),
+    (129, 20, 30, (BRIEF, BRIEF, NARROW_B))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n,ways", FEW_SHAPES)
+@pytest.mark.parametrize("act,residual", [(None, True), ("silu", False)])
+def test_gpu_linear_few(m, k, n, ways, act, residual):
+    from cpd_amd import ops
+    plan = ops.hip_ext().linear_plan(m, n, k, torch.float32, True, True)
+    assert tuple(plan[7:]) == ways
+    run_linear("cuda", torch.float32, m, k, n, act, residual)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n,ways", FEW_SHAPES)
+def test_gpu_linear_few_whole_numbers(m, k, n, ways):
+    """Every sum exact: equal to the formula in 64 bits, from strided and
+    misaligned operands too, and the gradients alone as together."""
+    g = torch.Generator(device="cuda").manual_seed(m + k + n)
+    draw = lambda *s: torch.randint(  # noqa: E731
+        -2, 3, s, generator=g, device="cuda").float()
+    b, res = draw(n) + 0.5, draw(m, n)
+    for pad, off in ((0, 0), (5, 3)):
+        x, w, dy = (draw(r, c + pad)[:, off:c + off]
+                    for r, c in ((m, k), (n, k), (m, n)))
+        x64, w64, dy64 = x.double(), w.double(), dy.double()
+        z = x64 @ w64.t() + b.double()
+        assert torch.equal(fused_linear(x, w, b, "relu", res),
+                           (z.clamp_min(0) + res.double()).float())
+        want = ((dy64 @ w64).float(), (dy64.t() @ x64).float(),
+                dy64.sum(0).float())
+        for need in ((True, True), (True, False), (False, True)):
+            leaves = [v.detach().requires_grad_(r)
+                      for v, r in zip((x, w, b), need + (need[0],))]
+            fused_linear(*leaves).backward(dy)
+            for v, c in zip(leaves, want):
+                assert v.grad is None or torch.equal(v.grad, c)
+
+
+@pytest.mark.gpu
+def test_gpu_linear_few_far_offsets():
+    """Operands and results whose offsets pass 2^31 elements, and 2^25 rows."""
+    for m, k, n in (((1 << 19) + 5, 4200, 8), ((1 << 19) + 5, 8, 4200),
+                    ((1 << 25) + 5, 4, 3)):
+        x, dy = (torch.zeros(m, c, device="cuda") for c in (k, n))
+        x[-3:] = torch.randint(-2, 3, (3, k), device="cuda").float()
+        dy[-3:] = torch.randint(-2, 3, (3, n), device="cuda").float()
+        w = torch.randint(-2, 3, (n, k), device="cuda").float()
+        x.requires_grad_(True)
+        w.requires_grad_(True)
+        y = fused_linear(x, w)
+        last, w64 = x.detach()[-3:].double(), w.detach().double()
+        assert torch.equal(y[-3:], (last @ w64.t()).float())
+        assert not y[:-3].any()
+        dx, dw = torch.autograd.grad(y, [x, w], dy)
+        assert torch.equal(dx[-3:], (dy[-3:].double() @ w64).float())
+        assert not dx[:-3].any()
+        assert torch.equal(dw, (dy[-3:].double().t().contiguous()
+                                @ last).float())
+        del x, dy, y, dx
+    # more rows than a launch of few features could take
+    x = torch.zeros((1 << 27) + 37, 33, device="cuda")
+    x[-3:] = 1
+    y = fused_linear(x, torch.ones(1, 33, device="cuda"))
+    assert (y[-3:] == 33).all() and not y[:-3].any()
+
+
+@pytest.mark.gpu
+def test_gpu_linear_few_not_finite():
+    """Infinities and NaN reach their own rows and columns and no others, and
+    what lies behind an operand's end reaches none."""
+    for m, k, n in ((200, 300, 9), (300, 20, 200), (5, 5000, 900)):
+        x = torch.ones(m, k, device="cuda")
+        w = torch.ones(n, k + 4, device="cuda")
+        w[:, k:] = math.nan
+        w = w[:, :k]
+        x[1, k - 1], x[m - 1, 0], w[2, 5] = math.inf, math.nan, -math.inf
+        y = fused_linear(x, w)
+        want = torch.full((m, n), float(k), device="cuda")
+        want[1] = math.inf
+        want[:, 2] = -math.inf
+        want[1, 2] = math.nan
+        want[m - 1] = math.nan
+        assert torch.equal(y.nan_to_num(1, 2, 3), want.nan_to_num(1, 2, 3))
+        a, b = (torch.ones(*s, device="cuda", requires_grad=True)
+                for s in ((m, k), (n, k)))
+        dy = torch.ones(m, n, device="cuda")
+        dy[3, n - 1] = math.inf
+        dx, dw = torch.autograd.grad(fused_linear(a, b), [a, b], dy)
+        assert dx.isinf().any(1).nonzero().flatten().tolist() == [3]
+        assert dw.isinf().any(1).nonzero().flatten().tolist() == [n - 1]
+        assert dx[3].isinf().all() and dw[n - 1].isinf().all()
+        assert not dx.isnan().any() and not dw.isnan().any()
