@@ -75,7 +75,13 @@ def fused_linear(x, weight, bias=None, activation=None, residual=None):
     2^-133, depending on the sizes.
 
     Rows may be apart by any stride; the result is contiguous.  Raises
-    TypeError and ValueError for types and shapes that do not fit.
+    TypeError and ValueError for types and shapes that do not fit, and on the
+    GPU for 2^22 features or more and 2^22 blocks of 128 by 128 or more in
+    ``x``, ``weight`` or the result.
+
+    On the GPU gradients are of first order: a graph of them
+    (``create_graph=True``) and forward-mode tangents raise RuntimeError.  On
+    CPU torch's own operations run, where both work.
     """
     if activation not in _ACTS:
         raise ValueError(f"unknown activation {activation!r}: None, 'relu', "

@@ -89,7 +89,13 @@ def fused_layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
     left out; their gradients come in their own type.  Rows of ``x`` may be
     apart by any stride (a slice of a wider tensor is read in place); results
     are contiguous.  Raises TypeError and ValueError for types and shapes that
-    do not fit.
+    do not fit, and on the GPU for 2^31 rows or more, or 2^22 of over 16384
+    elements.
+
+    On the GPU gradients are of first order: a graph of them
+    (``create_graph=True``) and forward-mode tangents raise RuntimeError.  On
+    CPU torch's own operations run, where both work, but for tangents beside a
+    ``residual``.
     """
     if not x.is_cuda:
         return _eager(x, weight, bias, eps, residual)

@@ -96,6 +96,10 @@ def token_logprobs(logits, targets, top_k=0, ignore_index=-100):
     Rows may be apart by any stride (``logits[..., :V]`` of a padded product
     is read in place).  Raises TypeError and ValueError for types and shapes
     that do not fit.
+
+    On the GPU gradients are of first order: a graph of them
+    (``create_graph=True``) and forward-mode tangents raise RuntimeError.  On
+    CPU torch's own operations run, where both work.
     """
     if not logits.is_cuda:
         return _eager(logits, targets, top_k, ignore_index)

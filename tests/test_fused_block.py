@@ -1958,3 +1958,34 @@ def test_gpu_linear_few_not_finite():
         assert dw.isinf().any(1).nonzero().flatten().tolist() == [n - 1]
         assert dx[3].isinf().all() and dw[n - 1].isinf().all()
         assert not dx.isnan().any() and not dw.isnan().any()
+
+
+def test_cpu_second_derivatives_and_tangents():
+    """What the docstrings say of the CPU path: second derivatives work, and
+    tangents but beside a norm's residual."""
+    from torch.autograd import forward_ad
+    g = rng(51)
+    x, w = (torch.randn(4, 16, generator=g) for _ in range(2))
+    t = torch.arange(4)
+    calls = [lambda v: fused_layer_norm(v, w[0]),
+             lambda v: fused_linear(v, w, None, "gelu"),
+             lambda v: token_logprobs(v, t).logprobs,
+             lambda v: token_logprobs(v, t).entropy]
+    for f in calls + [lambda v: fused_layer_norm(v, w[0], residual=w)[0]]:
+        leaf = x.clone().requires_grad_(True)
+        first, = torch.autograd.grad(f(leaf).square().sum(), leaf,
+                                     create_graph=True)
+        second, = torch.autograd.grad(first.square().sum(), leaf)
+        assert second.isfinite().all() and second.abs().sum() > 0
+    v = torch.randn(4, 16, generator=g)
+    for f in calls:
+        leaf = x.clone().requires_grad_(True)
+        want = (torch.autograd.grad(f(leaf).sum(), leaf)[0] * v).sum()
+        with forward_ad.dual_level():
+            got = forward_ad.unpack_dual(f(forward_ad.make_dual(x, v)))
+            torch.testing.assert_close(got.tangent.sum(), want, rtol=1e-3,
+                                       atol=1e-5)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, v)
+        with pytest.raises(RuntimeError):
+            fused_layer_norm(dual, w[0], residual=w)
