@@ -585,7 +585,8 @@ __global__ __launch_bounds__(256) void logprob_bwd_kernel(LogprobGradArgs a,
     const float logs = logf(sum), one = 1.f / sum;
     float glp = a.glogprobs ? a.glogprobs[row] : 0.f;
     const float gent = a.gentropy ? a.gentropy[row] : 0.f;
-    if (target < 0 || target >= a.vocab) glp = NAN;
+    // (the entropy does not ask for the target)
+    if ((target < 0 || target >= a.vocab) && a.glogprobs) glp = NAN;
     const float c0 = -(glp + gent * (a.gentropy ? a.entropy[row] : 0.f));
     // (all of a job's loads in flight at once: none under a condition but at a
     // row's end, and none across them)

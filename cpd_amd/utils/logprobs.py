@@ -90,8 +90,9 @@ def token_logprobs(logits, targets, top_k=0, ignore_index=-100):
     * NaN or +inf in a row makes its log probabilities, entropy and gradient
       NaN.  Among the alternatives NaN counts as the largest.
     * A target that is neither an index of the row nor ``ignore_index`` gives
-      NaN, in the log probability and in the row's gradient: targets are not
-      read on the host.
+      NaN, in the log probability and, where that is used, in the row's
+      gradient (the entropy's alone stays what it is): targets are not read on
+      the host.
 
     Rows may be apart by any stride (``logits[..., :V]`` of a padded product
     is read in place).  Raises TypeError and ValueError for types and shapes

@@ -1989,3 +1989,27 @@ def test_cpu_second_derivatives_and_tangents():
         dual = forward_ad.make_dual(x, v)
         with pytest.raises(RuntimeError):
             fused_layer_norm(dual, w[0], residual=w)
+
+
+@on_devices
+@pytest.mark.parametrize("vocab", [11, 5000])
+def test_logprobs_target_outside(device, vocab):
+    """A target outside the row: NaN where the log probability is used, and
+    the entropy and its own gradient as with any target."""
+    x, _ = make_logits(rng(vocab, 61), torch.float32, device, 3, vocab)
+    bad = torch.tensor([vocab, -1, 2 ** 40]).to(device)
+    good = torch.zeros(3, dtype=torch.int64, device=device)
+    got = []
+    for t in (bad, good):
+        leaf = x.to(device).requires_grad_(True)
+        out = token_logprobs(leaf, t)
+        ent, = torch.autograd.grad(out.entropy.sum(), leaf, retain_graph=True)
+        lp, = torch.autograd.grad(out.logprobs.sum(), leaf, retain_graph=True)
+        both, = torch.autograd.grad((out.entropy + 0 * out.logprobs).sum(),
+                                    leaf)
+        got.append((out, ent, lp, both))
+    (a, ent_a, lp_a, both_a), (b, ent_b, lp_b, _) = got
+    assert a.logprobs.isnan().all() and b.logprobs.isfinite().all()
+    assert torch.equal(a.entropy, b.entropy) and torch.equal(ent_a, ent_b)
+    assert lp_a.isnan().all() and both_a.isnan().all()
+    assert lp_b.isfinite().all()
