@@ -195,7 +195,7 @@ __device__ __forceinline__ s16x8 fragment(const char* half, int row, int kk,
 // nine products of two floats' parts the six largest are kept,
 //   a1 b1 + (a1 b2 + a2 b1) + (a1 b3 + a2 b2 + a3 b1),
 // the rest is below 2^-24 of a b.  A sixth of the 16-bit rate is 0.42 PFLOP/s
-// against the float matrix instructions' 0.157; 0.20 are measured at 8192 x 2048
+// against the float matrix instructions' 0.157; 0.21 are measured at 8192 x 2048
 // by 8192, where the library's float product has 0.15.
 //
 // Where a 16-bit product gets one operand in floats (dz), both are cut into two

@@ -11,7 +11,7 @@
 // accumulators before the one rounding to the output's type.
 //
 // bf16 at 8192^3: 1.46 PFLOP/s forward, 1.32 dx, 1.31 dW (the library's plain
-// product: 1.48, 1.39, 1.20); 2048^3: 0.76; floats at 8192 x 2048 x 8192: 0.20.
+// product: 1.48, 1.39, 1.20); 2048^3: 0.83; floats at 8192 x 2048 x 8192: 0.21.
 #include <type_traits>
 #include <utility>
 
@@ -726,7 +726,8 @@ __global__ __launch_bounds__(512) void gemm_rows_kernel(GemmArgs g) {
 // groups of lanes off each other's banks.
 //
 // Bound by reading many: 590 MB, 16384 x 9000 to 8, take 103 us forward and 110 for
-// dW (5.7 and 5.4 TB/s; by tiles 182 and 202).
+// dW (5.7 and 5.4 TB/s; by tiles 182 and 202; 186 where dW follows dx, whose writes
+// drain meanwhile).
 template <int RS, int K, bool ACROSS>
 struct NarrowStager {  // a thread's share of RS rows by K k
   static constexpr int CHUNKS = RS * K / 4;
@@ -904,7 +905,8 @@ __global__ __launch_bounds__(512) void gemm_narrow_kernel(GemmArgs g) {
 // rows in registers and goes down `rows_per` rows of A, sixteen at a time, the next
 // ones in flight; it has no LDS and no barrier, so that waves write while others
 // load.  A lane's elements of a sum are 4 Q (lane / 16) and on.  16384 x 9000 out of
-// sums of 8, 590 MB: 190 us (by tiles 245).
+// sums of 8, 590 MB: 126 us in a training step (4.7 TB/s), 190 one after the other
+// (by tiles 245).
 template <int Q, bool AX, bool BX>
 __global__ __launch_bounds__(256) void gemm_short_kernel(GemmArgs g, int rows_per) {
   constexpr int N = 4 * Q;

@@ -22,10 +22,11 @@
 // k log(n / k) times in n values; values that keep rising pass often, which is
 // slower but as right.
 //
-// Without alternatives 4096 rows of 50021 bf16 take 95 us (4.3 TB/s) forward and
-// 149 backward (5.5 TB/s).  Alternatives add work: 2048 rows of 131072 fp16 take
-// 99 us, 121 with one, 143 with five, 169 with sixteen, 224 with 64 (inserted one
-// by one 123, 154, 195 and 305).
+// Calls one after the other, three inputs in turn: without alternatives 4096 rows of
+// 50021 bf16 take 93 us (4.4 TB/s) forward and 152 backward (5.4 TB/s); in a training
+// step, behind each other's writes, 110 to 120 and 139 to 165.  Alternatives add
+// work: 2048 rows of 131072 fp16 take 98 us, 121 with one, 144 with five, 171 with
+// sixteen, 228 with 64 (inserted one by one 123, 154, 195 and 305).
 //
 // A row of -inf alone has log probability -inf, entropy 0 and no gradient.
 // NaN or +inf in a row makes its log probabilities NaN; among the
@@ -102,7 +103,7 @@ __device__ __forceinline__ Soft join(Soft v, Soft o) {
 }
 
 // The same over a wave: the maximum first, so that each lane rescales once
-// (32768 rows of 1000 floats: 27 us; pair by pair through LDS 31).
+// (32768 rows of 1000 floats: 32 us; pair by pair through LDS 4 more).
 __device__ __forceinline__ Soft wave_join(Soft v) {
   const float m = group_max(v.m);
   const bool none = v.m == -INFINITY;

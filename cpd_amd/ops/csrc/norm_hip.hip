@@ -16,7 +16,7 @@
 //
 // With bf16 rows of 4096 and the residual, 8192 of them take 60 us forward and
 // 61 + 4 backward (268 MB each: 4.5 and 4.1 TB/s, where a copy of 1 GiB runs at
-// 4.9); 20011 float rows of 257 take 12 and 18 + 4 (3.3 and 2.8 TB/s).
+// 4.95); 20011 float rows of 257 take 12 and 18 + 4 (3.3 and 2.8 TB/s).
 #include "fused_ops.h"
 
 namespace cpd {
