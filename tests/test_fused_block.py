@@ -1702,7 +1702,10 @@ class WithoutMemory(torch.Tensor):
 def test_refuses_inputs_without_memory():
     """Before anything is asked of a GPU."""
     from cpd_amd import ops
-    ext = ops.hip_ext()
+    try:
+        ext = ops.hip_ext()
+    except RuntimeError:
+        pytest.skip("the HIP extension is not built")
     x = WithoutMemory(torch.zeros(4, 16))
     t = torch.zeros(4, dtype=torch.int64)
     for call in (lambda: ext.layer_norm(x, None, None, 1e-5, None),
