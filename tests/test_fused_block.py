@@ -2016,3 +2016,42 @@ def test_logprobs_target_outside(device, vocab):
     assert torch.equal(a.entropy, b.entropy) and torch.equal(ent_a, ent_b)
     assert lp_a.isnan().all() and both_a.isnan().all()
     assert lp_b.isfinite().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(5003, 200, 7), (70, 9001, 20),
+                                   (3, 4900, 1003), (700, 25, 4703)])
+def test_gpu_linear_few_captured(m, k, n):
+    """Forward and backward of few features, slices and their joining among
+    them, in two graphs that are replayed in turn, with eager work between the
+    replays."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    draw = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    inputs = [[draw(m, k), draw(n, k), draw(n), draw(m, n)] for _ in range(3)]
+
+    def step(x, w, b, dy):
+        leaves = [v.detach().requires_grad_(True) for v in (x, w, b)]
+        y = fused_linear(*leaves, "gelu")
+        return [v.detach() for v in (y, *torch.autograd.grad(y, leaves, dy))]
+
+    want = [step(*v) for v in inputs]
+    graphs = []
+    for _ in range(2):
+        static = [v.clone() for v in inputs[0]]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(*static)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*static)
+        graphs.append((graph, static, out))
+    for i in range(6):
+        graph, static, out = graphs[i % 2]
+        for a, b in zip(static, inputs[i % 3]):
+            a.copy_(b)
+        graph.replay()
+        step(*inputs[(i + 1) % 3])
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want[i % 3]))
